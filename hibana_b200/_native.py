@@ -7,6 +7,7 @@ suite exercises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import threading
 from ctypes import c_float, c_int, c_longlong, c_void_p
@@ -138,6 +139,15 @@ def stream() -> int:
     a `torch.cuda.Stream` object first took 15, a fifth of the time an eager prefill spends launching."""
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
+
+def on_device(t: torch.Tensor):
+    """Context in which `t`'s device is the current one: launches and `stream()` go there. Costs nothing where it is already."""
+    if t.device.index == torch._C._cuda_getDevice():
+        return _HERE
+    return torch.cuda.device(t.device)
+
+
+_HERE = contextlib.nullcontext()
 
 CALLS = 0      # native entry points called
 LAUNCHES = 0   # kernels those calls launched (each call launches at least one)

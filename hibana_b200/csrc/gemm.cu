@@ -5,6 +5,9 @@
 //                  256-element (128-byte) K tiles; scale factors travel global -> shared by bulk copies of the
 //                  128x4-swizzled blocks and shared -> TMEM by tcgen05.cp.
 //
+//   * kind mxfp4 : tcgen05.mma kind::mxf4.block_scale (e2m1 values, ue8m0 scale per 32 elements): the same tiles with half as
+//                  many scale bytes.
+//
 //   * kind fp8   : tcgen05.mma kind::f8f6f4 on e4m3 operands, 128-element (128-byte) K tiles; per-tensor scales
 //                  fold into alpha, a per-token scale vector (dynamic activation quantisation) into the epilogue.
 //   * kind w3    : the A operand is a 3-bit weight copy (asymmetric integer codes, groups of 64 along K, bf16 scale
@@ -50,8 +53,9 @@ template <int KIND, int BN>
 struct Cfg {
   static constexpr int B_TILE_BYTES = BN * ROW_BYTES;
   static constexpr int NRB = (BN + 127) / 128;
-  static constexpr int SFA_BYTES = KIND == kGemmNvfp4 ? 4 * 512 : 0;
-  static constexpr int SFB_BYTES = KIND == kGemmNvfp4 ? NRB * 4 * 512 : 0;
+  static constexpr int ATOMS = sf_atoms(KIND);
+  static constexpr int SFA_BYTES = ATOMS * 512;
+  static constexpr int SFB_BYTES = NRB * ATOMS * 512;
   static constexpr int PACK_BYTES = KIND == kGemmW3 ? 4096 : 0;   // packed 3-bit tile, behind the operand tiles
   static constexpr int STAGE_BYTES = A_TILE_BYTES + B_TILE_BYTES + SFA_BYTES + SFB_BYTES + PACK_BYTES;
   static constexpr int TX_BYTES = KIND == kGemmW3 ? B_TILE_BYTES + PACK_BYTES : STAGE_BYTES;   // bytes copies deliver
@@ -63,7 +67,7 @@ struct Cfg {
   static constexpr int SMEM_BUDGET = BN <= 64 ? 100 * 1024 : BN == 128 ? 110 * 1024 : 200 * 1024;
   static constexpr int STAGES_RAW = SMEM_BUDGET / STAGE_BYTES;
   static constexpr int STAGES = STAGES_RAW > 8 ? 8 : STAGES_RAW;
-  static constexpr int TMEM_NEED = BN + (KIND == kGemmNvfp4 ? 16 + 16 * NRB : 0);
+  static constexpr int TMEM_NEED = BN + (is_fp4(KIND) ? 16 + 16 * NRB : 0);
   static constexpr int TMEM_COLS =
       TMEM_NEED <= 32 ? 32 : TMEM_NEED <= 64 ? 64 : TMEM_NEED <= 128 ? 128 : TMEM_NEED <= 256 ? 256 : 512;
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256;
@@ -501,16 +505,16 @@ gemm_kernel(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUt
           return;
         }
         tma_load_2d(st, &tma, bar, kx, ua_row0);
-        if constexpr (KIND == kGemmNvfp4)
+        if constexpr (is_fp4(KIND))
           bulk_load(st + A_TILE_BYTES + C::B_TILE_BYTES,
-                    p.sfa + (static_cast<size_t>(ua_row0 >> 7) * p.ka_a + kt * 4) * 512, 2048, bar);
+                    p.sfa + (static_cast<size_t>(ua_row0 >> 7) * p.ka_a + kt * C::ATOMS) * 512, C::SFA_BYTES, bar);
       } else {
         tma_load_2d(st + A_TILE_BYTES, &tmb, bar, kx, ub_row0);
-        if constexpr (KIND == kGemmNvfp4) {
+        if constexpr (is_fp4(KIND)) {
 #pragma unroll
           for (int rb = 0; rb < C::NRB; ++rb)
-            bulk_load(st + A_TILE_BYTES + C::B_TILE_BYTES + C::SFA_BYTES + rb * 2048,
-                      p.sfb + (static_cast<size_t>((ub_row0 >> 7) + rb) * p.ka_b + kt * 4) * 512, 2048, bar);
+            bulk_load(st + A_TILE_BYTES + C::B_TILE_BYTES + C::SFA_BYTES + rb * C::SFA_BYTES,
+                      p.sfb + (static_cast<size_t>((ub_row0 >> 7) + rb) * p.ka_b + kt * C::ATOMS) * 512, C::SFA_BYTES, bar);
         }
       }
     };
@@ -627,6 +631,20 @@ gemm_kernel(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUt
           for (int kb = 0; kb < 4; ++kb)
             mma_nvf4(tmem_base, adesc + kb * 2, bdesc + kb * 2, idesc, (i > 0 || kb > 0) ? 1u : 0u,
                      sfa_t + kb * 4, sfb_t + kb * 4 * C::NRB);
+        } else if constexpr (KIND == kGemmMxfp4) {
+          const uint32_t sf = st + A_TILE_BYTES + C::B_TILE_BYTES;
+#pragma unroll
+          for (int at = 0; at < 2; ++at) {
+            tmem_cp_32x128b_x4(sfa_t + at * 4, make_desc_sf(sf + at * 512));
+#pragma unroll
+            for (int rb = 0; rb < C::NRB; ++rb)
+              tmem_cp_32x128b_x4(sfb_t + at * 4 * C::NRB + rb * 4,
+                                 make_desc_sf(sf + C::SFA_BYTES + rb * C::SFA_BYTES + at * 512));
+          }
+#pragma unroll
+          for (int kb = 0; kb < 4; ++kb)       // an atom holds the scales of two instructions
+            mma_mxf4(tmem_base, adesc + kb * 2, bdesc + kb * 2, make_idesc_mxf4(BM, BN, kb & 1), (i > 0 || kb > 0) ? 1u : 0u,
+                     sfa_t + (kb >> 1) * 4, sfb_t + (kb >> 1) * 4 * C::NRB);
         } else if constexpr (KIND == kGemmFp8) {
 #pragma unroll
           for (int kb = 0; kb < 4; ++kb)
@@ -987,7 +1005,7 @@ template <int KIND, int BN>
 cudaError_t launch_t(const GemmArgs& a, DevParams& p, dim3 grid, const CUtensorMap* ta, const CUtensorMap* tb,
                      cudaStream_t stream) {
   using C = Cfg<KIND, BN>;
-  constexpr int K_ELEMS = KIND == kGemmNvfp4 ? 256 : KIND == kGemmFp8 ? 128 : 64;      // of a K tile
+  constexpr int K_ELEMS = is_fp4(KIND) ? 256 : KIND == kGemmFp8 ? 128 : 64;      // of a K tile
   static bool attr_done = false;
   static int max_clusters[9] = {0, 0, 0, 0, 0, 0, 0, 0, 0};   // co-resident clusters per cluster size (0 = unknown)
   if (!attr_done) {
@@ -1107,7 +1125,7 @@ size_t gemm_workspace_bytes(const GemmArgs& a) {
 int gemm_num_tiles(const GemmArgs& a) { return ((a.ra + BM - 1) / BM) * ((a.rb + a.bn - 1) / a.bn); }
 
 cudaError_t gemm_launch(const GemmArgs& a, cudaStream_t stream) {
-  const bool fp4 = a.kind == kGemmNvfp4;
+  const bool fp4 = is_fp4(a.kind);
   const bool fp8 = a.kind == kGemmFp8;
   const bool w3 = a.kind == kGemmW3;
   if (a.ra <= 0 || a.rb <= 0 || a.k <= 0) return cudaErrorInvalidValue;
@@ -1122,7 +1140,11 @@ cudaError_t gemm_launch(const GemmArgs& a, cudaStream_t stream) {
     return cudaErrorInvalidValue;
   if (fp4 && a.bn < 128 && tiles_b != 1 && !grouped) return cudaErrorInvalidValue;
   if (fp4 && grouped && a.bn < 128 && a.grp_chunks != 1) return cudaErrorInvalidValue;
-  if (fp4 && (a.sf_k_atoms_a < k_tiles * 4 || a.sf_k_atoms_b < k_tiles * 4)) return cudaErrorInvalidValue;
+  const int atoms = k_tiles * sf_atoms(a.kind);
+  if (fp4 && (a.sf_k_atoms_a < atoms || a.sf_k_atoms_b < atoms)) return cudaErrorInvalidValue;
+  // the requantising epilogues write NVFP4 for an NVFP4 product
+  if (a.kind == kGemmMxfp4 && (a.epilogue == kEpiSiluMulQuant || a.epilogue == kEpiRelu2Quant || a.peer != nullptr || a.ep != nullptr))
+    return cudaErrorInvalidValue;
   int splits = a.splits == 0 || grouped ? 1 : std::abs(a.splits);      // negative: see launch_t
   if (splits > k_tiles) splits = k_tiles;
   // Every split must own at least one K tile.
@@ -1224,7 +1246,9 @@ cudaError_t gemm_launch(const GemmArgs& a, cudaStream_t stream) {
     case 256: return launch_t<KIND, 256>(a, p, grid, ta, tb, stream);            \
     default: return cudaErrorInvalidValue;                                       \
   }
-  if (fp4) {
+  if (a.kind == kGemmMxfp4) {
+    HB_DISPATCH(kGemmMxfp4)
+  } else if (fp4) {
     HB_DISPATCH(kGemmNvfp4)
   } else if (fp8) {
     HB_DISPATCH(kGemmFp8)

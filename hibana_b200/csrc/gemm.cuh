@@ -12,7 +12,11 @@ enum GemmKind : int {
   kGemmFp8 = 2,   // e4m3 x e4m3, 128-element K tiles
   kGemmW3 = 3,    // A = 3-bit asymmetric codes (groups of 64, bf16 scale + zero) in 4096-byte tiles, dequantised to
                   // bf16 in shared memory by the CTA; B = bf16 activations; weights on the 128-row side only
+  kGemmMxfp4 = 4, // e2m1 x e2m1, one ue8m0 scale per 32 elements
 };
+constexpr bool is_fp4(int kind) { return kind == kGemmNvfp4 || kind == kGemmMxfp4; }
+// Scale atoms (512-byte blocks: 128 rows x 4 scales) of a 256-element K tile: 64 elements each for nvfp4, 128 for mxfp4.
+constexpr int sf_atoms(int kind) { return kind == kGemmNvfp4 ? 4 : kind == kGemmMxfp4 ? 2 : 0; }
 enum GemmEpilogue : int {
   kEpiStore = 0,      // out = alpha * acc                      (bf16)
   kEpiResidual = 1,   // out = alpha * acc + residual           (bf16)
@@ -65,8 +69,8 @@ struct GemmArgs {
   int kind;
   const void* a;        // [RA, K]  (bf16, or packed e2m1 with K/2 bytes per row)
   const void* b;        // [RB, K]
-  const void* sfa;      // nvfp4 only: scale factors of A, 128x4-swizzled blocks [ceil(RA/128)][KA][512 B]
-  const void* sfb;      // nvfp4 only: scale factors of B
+  const void* sfa;      // nvfp4 / mxfp4: scale factors of A, 128x4-swizzled blocks [ceil(RA/128)][KA][512 B]
+  const void* sfb;      // nvfp4 / mxfp4: scale factors of B
   int ra, rb, k;
   int64_t lda, ldb;     // row pitch in elements
   void* out;
@@ -81,7 +85,7 @@ struct GemmArgs {
   int* counters;        // splits > 1: one int per output tile, zero before the first launch, self-resetting
   int* status;          // device status word (may be null)
   int bn;               // N tile: 16, 32, 64, 128 or 256
-  int sf_k_atoms_a;     // nvfp4: number of 64-element K atoms per row block in sfa (padded to a multiple of 4)
+  int sf_k_atoms_a;     // number of K atoms per row block in sfa, padded to whole K tiles (see sf_atoms)
   int sf_k_atoms_b;
   // grouped mode (null grp_cnt = off); see hb_gemm_grouped
   const int* grp_start;

@@ -1,4 +1,6 @@
-// Prefill-sized NVFP4 GEMM for sm_100a on SM pairs: D[m, n] = A[m, K] * B[n, K]^T, tokens on the A side.
+// Prefill-sized NVFP4 / MXFP4 GEMM for sm_100a on SM pairs: D[m, n] = A[m, K] * B[n, K]^T, tokens on the A side.
+//
+// (Both formats run the same kernel; an mxfp4 K tile has half as many scale bytes.)
 //
 // Two CTAs of a cluster share one 256 x 256 output tile (tcgen05 cta_group::2, M = 256): each stages its own 128 rows
 // of A and HALF of B, and the leader's MMA reads both shared memories. A 128 x 256 tile on one SM has to read
@@ -46,12 +48,16 @@ constexpr int THREADS = 64 + EPI_WARPS * 32;  // producer warp, MMA warp, epilog
 constexpr int STAGES = 5;
 constexpr int A_BYTES = 128 * 128;            // 128 rows x 256 packed e2m1
 constexpr int B_BYTES = 128 * 128;            // this CTA's half of the 256 columns
-constexpr int SFA_BYTES = 2048;               // one 128-row block x 4 K atoms
-constexpr int SFB_BYTES = 4096;               // two 128-column blocks x 4 K atoms (each CTA holds all columns' scales)
-constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES;
 constexpr int ROW_PITCH = 80;                 // staged output row: 64 bytes (conflict-free 16-byte accesses)
 constexpr int STAGING_BYTES = EPI_WARPS * 32 * ROW_PITCH;
-constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + STAGING_BYTES + 256;
+template <int KIND>
+struct PairCfg {
+  static constexpr int ATOMS = sf_atoms(KIND);            // scale atoms of a K tile: 4 (nvfp4) or 2 (mxfp4)
+  static constexpr int SFA_BYTES = ATOMS * 512;           // one 128-row block
+  static constexpr int SFB_BYTES = 2 * ATOMS * 512;       // two 128-column blocks (each CTA holds all columns' scales)
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES;
+  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + STAGING_BYTES + 256;
+};
 constexpr int ACC1_COL = 208;                 // first column of the second accumulator
 constexpr int SFA_COL = 464;                  // 4 K atoms x 4 columns
 constexpr int SFB_COL = 480;                  // 4 K atoms x 8 columns
@@ -202,6 +208,15 @@ __device__ __forceinline__ void mma_nvf4_pair(uint32_t d_tmem, uint64_t adesc, u
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(sfa_tmem), "r"(sfb_tmem)
       : "memory");
 }
+__device__ __forceinline__ void mma_mxf4_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                              uint32_t accumulate, uint32_t sfa_tmem, uint32_t sfb_tmem) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.block32 [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(
+          d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(sfa_tmem), "r"(sfb_tmem)
+      : "memory");
+}
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
@@ -340,12 +355,14 @@ __device__ __forceinline__ void epilogue_unit(const PairParams& p, const Unit& x
   }
 }
 
-template <int EPI, bool GRP>
+template <int KIND, int EPI, bool GRP>
 __global__ void __launch_bounds__(THREADS, 1)
 gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap ta64,
                  const __grid_constant__ CUtensorMap ta32, const __grid_constant__ CUtensorMap tb,
                  const __grid_constant__ CUtensorMap tb_sub, const __grid_constant__ CUtensorMap tsfa,
                  const __grid_constant__ CUtensorMap tsfb, const PairParams p) {
+  using C = PairCfg<KIND>;
+  constexpr int SFA_BYTES = C::SFA_BYTES, SFB_BYTES = C::SFB_BYTES, STAGE_BYTES = C::STAGE_BYTES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* staging = smem + STAGES * STAGE_BYTES;
@@ -402,13 +419,13 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__
       if (GRP && box == 0) return;
       tma_load_2d_pair(st, !GRP || box == 128 ? &ta : box == 64 ? &ta64 : &ta32, full0 + s * 8, kt * 128,
                        x.m0 + static_cast<int>(rank) * 128);
-      tma_load_2d_pair(st + A_BYTES + B_BYTES, &tsfa, full0 + s * 8, kt * 256, (x.m0 >> 7) + static_cast<int>(rank));
+      tma_load_2d_pair(st + A_BYTES + B_BYTES, &tsfa, full0 + s * 8, kt * C::ATOMS * 64, (x.m0 >> 7) + static_cast<int>(rank));
     };
     auto side_b = [&](const Unit& x, int kt, int s) {
       const uint32_t st = smem_base + s * STAGE_BYTES;
       tma_load_2d_pair(st + A_BYTES, x.width == PAIR_N ? &tb : &tb_sub, full0 + s * 8, kt * 128,
                        x.b0 + static_cast<int>(rank) * (x.width >> 1));
-      tma_load_2d_pair(st + A_BYTES + B_BYTES + SFA_BYTES, &tsfb, full0 + s * 8, kt * 256, x.b0 >> 7);
+      tma_load_2d_pair(st + A_BYTES + B_BYTES + SFA_BYTES, &tsfb, full0 + s * 8, kt * C::ATOMS * 64, x.b0 >> 7);
     };
     auto tx_bytes = [&](const Unit& x) {
       uint32_t bytes = 2u * (SFB_BYTES + static_cast<uint32_t>(x.width) * 64u);
@@ -509,15 +526,20 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__
           const uint32_t sf = st + A_BYTES + B_BYTES;
           if (elect_one()) {
 #pragma unroll
-            for (int kb = 0; kb < 4; ++kb) {
-              tmem_cp_32x128b_x4_pair(sfa_t + kb * 4, make_desc_sf(sf + kb * 512));
-              tmem_cp_32x128b_x4_pair(sfb_t + kb * 8, make_desc_sf(sf + SFA_BYTES + kb * 512));
-              tmem_cp_32x128b_x4_pair(sfb_t + kb * 8 + 4, make_desc_sf(sf + SFA_BYTES + 2048 + kb * 512));
+            for (int at = 0; at < C::ATOMS; ++at) {
+              tmem_cp_32x128b_x4_pair(sfa_t + at * 4, make_desc_sf(sf + at * 512));
+              tmem_cp_32x128b_x4_pair(sfb_t + at * 8, make_desc_sf(sf + SFA_BYTES + at * 512));
+              tmem_cp_32x128b_x4_pair(sfb_t + at * 8 + 4, make_desc_sf(sf + SFA_BYTES + SFA_BYTES + at * 512));
             }
 #pragma unroll
-            for (int kb = 0; kb < 4; ++kb)
-              mma_nvf4_pair(acc, adesc + kb * 2, bdesc + kb * 2, idesc, (kt > 0 || kb > 0) ? 1u : 0u, sfa_t + kb * 4,
-                            sfb_u + kb * 8);
+            for (int kb = 0; kb < 4; ++kb) {
+              if constexpr (KIND == kGemmNvfp4)
+                mma_nvf4_pair(acc, adesc + kb * 2, bdesc + kb * 2, idesc, (kt > 0 || kb > 0) ? 1u : 0u, sfa_t + kb * 4,
+                              sfb_u + kb * 8);
+              else                       // an atom holds the scales of two instructions
+                mma_mxf4_pair(acc, adesc + kb * 2, bdesc + kb * 2, idesc | make_idesc_mxf4(0, 0, kb & 1),
+                              (kt > 0 || kb > 0) ? 1u : 0u, sfa_t + (kb >> 1) * 4, sfb_u + (kb >> 1) * 8);
+            }
             tc_commit_pair(&empty[s]);
             if (kt == p.k_tiles - 1) tc_commit_pair(&accum[it & 1]);
           }
@@ -557,14 +579,14 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__
   if (warp == 1) tmem_dealloc_pair(tmem_base, 512);
 }
 
-template <int EPI, bool GRP>
+template <int KIND, int EPI, bool GRP>
 cudaError_t launch(const CUtensorMap& ta, const CUtensorMap& ta64, const CUtensorMap& ta32, const CUtensorMap& tb,
                    const CUtensorMap& tb_sub, const CUtensorMap& tsfa, const CUtensorMap& tsfb, const PairParams& p, int clusters,
                    cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * clusters);
   cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = SMEM_BYTES;
+  cfg.dynamicSmemBytes = PairCfg<KIND>::SMEM_BYTES;
   cfg.stream = stream;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -573,26 +595,26 @@ cudaError_t launch(const CUtensorMap& ta, const CUtensorMap& ta64, const CUtenso
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = hb_gemm_get_pdl() && !hb_take_plain() ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, gemm_pair_kernel<EPI, GRP>, ta, ta64, ta32, tb, tb_sub, tsfa, tsfb, p);
+  return cudaLaunchKernelEx(&cfg, gemm_pair_kernel<KIND, EPI, GRP>, ta, ta64, ta32, tb, tb_sub, tsfa, tsfb, p);
 }
 
 // Clusters of two that the device holds at once (0 = the kernels could not be set up).
-template <int EPI, bool GRP>
+template <int KIND, int EPI, bool GRP>
 int resident_clusters() {
-  if (cudaFuncSetAttribute(gemm_pair_kernel<EPI, GRP>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) !=
-      cudaSuccess)
+  if (cudaFuncSetAttribute(gemm_pair_kernel<KIND, EPI, GRP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           PairCfg<KIND>::SMEM_BYTES) != cudaSuccess)
     return 0;
   cudaLaunchConfig_t q = {};
   q.gridDim = dim3(2);
   q.blockDim = dim3(THREADS);
-  q.dynamicSmemBytes = SMEM_BYTES;
+  q.dynamicSmemBytes = PairCfg<KIND>::SMEM_BYTES;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
   q.attrs = at;
   q.numAttrs = 1;
   int n = 0;
-  if (cudaOccupancyMaxActiveClusters(&n, gemm_pair_kernel<EPI, GRP>, &q) != cudaSuccess) {
+  if (cudaOccupancyMaxActiveClusters(&n, gemm_pair_kernel<KIND, EPI, GRP>, &q) != cudaSuccess) {
     (void)cudaGetLastError();
     return 0;
   }
@@ -602,8 +624,9 @@ int resident_clusters() {
 }  // namespace
 
 bool gemm_pair_ok(const GemmArgs& a) {
-  if (a.kind != kGemmNvfp4 || a.peer != nullptr || a.ep != nullptr || a.tok_scale != nullptr || a.bn != 256) return false;
+  if (!is_fp4(a.kind) || a.peer != nullptr || a.ep != nullptr || a.tok_scale != nullptr || a.bn != 256) return false;
   const bool grouped = a.grp_cnt != nullptr;
+  if (a.kind == kGemmMxfp4 && grouped) return false;
   if (grouped) {
     if (!a.swap || a.grp_tiles == nullptr || a.grp_rows_a % 128 != 0) return false;
   } else if (a.swap || a.splits > 1) {
@@ -619,15 +642,22 @@ bool gemm_pair_ok(const GemmArgs& a) {
 }
 
 cudaError_t gemm_pair_launch(const GemmArgs& a, cudaStream_t stream) {
-  static const int resident = [] {
-    int n = resident_clusters<kEpiStore, false>();
-    n = std::min(n, resident_clusters<kEpiResidual, false>());
-    n = std::min(n, resident_clusters<kEpiSiluMul, false>());
-    n = std::min(n, resident_clusters<kEpiSiluMulQuant, false>());
-    n = std::min(n, resident_clusters<kEpiStore, true>());
-    n = std::min(n, resident_clusters<kEpiRelu2Quant, true>());
-    return std::min(n, resident_clusters<kEpiSiluMulQuant, true>());
+  static const int resident_nv = [] {
+    int n = resident_clusters<kGemmNvfp4, kEpiStore, false>();
+    n = std::min(n, resident_clusters<kGemmNvfp4, kEpiResidual, false>());
+    n = std::min(n, resident_clusters<kGemmNvfp4, kEpiSiluMul, false>());
+    n = std::min(n, resident_clusters<kGemmNvfp4, kEpiSiluMulQuant, false>());
+    n = std::min(n, resident_clusters<kGemmNvfp4, kEpiStore, true>());
+    n = std::min(n, resident_clusters<kGemmNvfp4, kEpiRelu2Quant, true>());
+    return std::min(n, resident_clusters<kGemmNvfp4, kEpiSiluMulQuant, true>());
   }();
+  static const int resident_mx = [] {
+    int n = resident_clusters<kGemmMxfp4, kEpiStore, false>();
+    n = std::min(n, resident_clusters<kGemmMxfp4, kEpiResidual, false>());
+    return std::min(n, resident_clusters<kGemmMxfp4, kEpiSiluMul, false>());
+  }();
+  const bool mx = a.kind == kGemmMxfp4;
+  const int resident = mx ? resident_mx : resident_nv;
   if (resident < 1) return cudaErrorInvalidConfiguration;
   const bool grouped = a.grp_cnt != nullptr;
   // tokens are the A side here; a grouped call names its weights first
@@ -689,8 +719,9 @@ cudaError_t gemm_pair_launch(const GemmArgs& a, cudaStream_t stream) {
   const TmapKey kb_sub{wgt, static_cast<uint64_t>(wgt_rows), cols, pitch_b, sub_rows, 128, 1};
   // scale factors as rows of 128-row blocks: 64 8-byte words per K atom
   const uint64_t pa = static_cast<uint64_t>(act_ka) * 512, pb = static_cast<uint64_t>(wgt_ka) * 512;
-  const TmapKey ksa{act_sf, static_cast<uint64_t>((rows + 127) / 128), pa / 8, pa, 1, 256, 2};
-  const TmapKey ksb{wgt_sf, static_cast<uint64_t>((wgt_rows + 127) / 128), pb / 8, pb, 2, 256, 2};
+  const uint32_t sf_box = static_cast<uint32_t>(sf_atoms(a.kind) * 64);
+  const TmapKey ksa{act_sf, static_cast<uint64_t>((rows + 127) / 128), pa / 8, pa, 1, sf_box, 2};
+  const TmapKey ksb{wgt_sf, static_cast<uint64_t>((wgt_rows + 127) / 128), pb / 8, pb, 2, sf_box, 2};
   CUtensorMap ta, ta64, ta32, tb, tb_sub, tsfa, tsfb;
   TmapKey k64 = ka, k32 = ka;
   if (grouped) {
@@ -700,7 +731,14 @@ cudaError_t gemm_pair_launch(const GemmArgs& a, cudaStream_t stream) {
   if (!get_tmap_2d(ka, &ta) || !get_tmap_2d(k64, &ta64) || !get_tmap_2d(k32, &ta32) || !get_tmap_2d(kb, &tb) ||
       !get_tmap_2d(kb_sub, &tb_sub) || !get_tmap_2d(ksa, &tsfa) || !get_tmap_2d(ksb, &tsfb))
     return cudaErrorInvalidValue;
-#define HB_PAIR(EPI, GRP) launch<EPI, GRP>(ta, ta64, ta32, tb, tb_sub, tsfa, tsfb, p, clusters, stream)
+#define HB_PAIR_K(KIND, EPI, GRP) launch<KIND, EPI, GRP>(ta, ta64, ta32, tb, tb_sub, tsfa, tsfb, p, clusters, stream)
+#define HB_PAIR(EPI, GRP) HB_PAIR_K(kGemmNvfp4, EPI, GRP)
+  if (mx) switch (a.epilogue) {
+    case kEpiStore: return HB_PAIR_K(kGemmMxfp4, kEpiStore, false);
+    case kEpiResidual: return HB_PAIR_K(kGemmMxfp4, kEpiResidual, false);
+    case kEpiSiluMul: return HB_PAIR_K(kGemmMxfp4, kEpiSiluMul, false);
+    default: return cudaErrorInvalidValue;
+  }
   switch (a.epilogue) {
     case kEpiStore: return grouped ? HB_PAIR(kEpiStore, true) : HB_PAIR(kEpiStore, false);
     case kEpiResidual: return HB_PAIR(kEpiResidual, false);
@@ -710,6 +748,7 @@ cudaError_t gemm_pair_launch(const GemmArgs& a, cudaStream_t stream) {
     default: return cudaErrorInvalidValue;
   }
 #undef HB_PAIR
+#undef HB_PAIR_K
 }
 
 }  // namespace hb

@@ -8,7 +8,7 @@ extern "C" {
 #endif
 
 // ---- GEMM (gemm.cu) ------------------------------------------------------------------------------------
-// kind: 0 bf16, 1 nvfp4. D[ra, rb] = A[ra, K] . B[rb, K]^T; swap != 0 stores D transposed (out[rb][ra]).
+// kind: 0 bf16, 1 nvfp4, 4 mxfp4. D[ra, rb] = A[ra, K] . B[rb, K]^T; swap != 0 stores D transposed (out[rb][ra]).
 // epilogue: 0 store bf16, 1 + residual, 2 silu(gate)*up on pairwise-interleaved rows/cols, 3 store fp32.
 int hb_gemm(int kind, const void* a, const void* b, const void* sfa, const void* sfb, int ra, int rb, int k,
             long long lda, long long ldb, void* out, long long ldo, const void* residual, float alpha,
@@ -100,6 +100,11 @@ int hb_quant_nvfp4_rows(const void* x, long long ldx, int m, int k, int ka, cons
                         int mode, const void* src_rows, const void* total_rows, void* stream);
 int hb_norm_quant_nvfp4(const void* x, void* residual, const void* w, float eps, int gemma, int m, int k, int ka,
                         const void* gscale, void* q, void* sf, void* normed, void* stream);
+// MXFP4 (mxfp4.cu): x of type 0 bf16, 1 fp16, 2 fp32; ka = 2 * ceil(k / 256) scale atoms per row block. src_rows / total_rows
+// (may be null): rows with a negative entry and rows from *total_rows on stay unwritten; gather: row r comes from src_rows[r].
+int hb_quant_mxfp4(const void* x, int in_type, long long ldx, int m, int k, int ka, void* q, void* sf, const void* src_rows,
+                   const void* total_rows, int gather, void* stream);
+int hb_dequant_mxfp4(const void* q, const void* sf, int m, int k, int ka, void* out, int out_type, void* stream);
 int hb_quant_fp8_static(const void* x, long long n, const void* scale, void* q, void* stream);
 int hb_quant_fp8_rows(const void* x, int m, int k, void* q, void* scales, void* stream);
 

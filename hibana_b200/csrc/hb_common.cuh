@@ -404,6 +404,16 @@ __device__ __forceinline__ void mma_nvf4(uint32_t d_tmem, uint64_t adesc, uint64
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(sfa_tmem), "r"(sfb_tmem)
       : "memory");
 }
+// The same with ue8m0 scales, one per 32 elements: an instruction uses two of the four scale bytes of a row (make_idesc_mxf4).
+__device__ __forceinline__ void mma_mxf4(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                         uint32_t accumulate, uint32_t sfa_tmem, uint32_t sfb_tmem) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.block32 [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(
+          d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(sfa_tmem), "r"(sfb_tmem)
+      : "memory");
+}
 // Shared -> TMEM copy of one 32 x 128-bit block replicated to the four 32-lane quarters (scale factors).
 __device__ __forceinline__ void tmem_cp_32x128b_x4(uint32_t taddr, uint64_t sdesc) {
   asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
@@ -506,6 +516,12 @@ __host__ __device__ constexpr uint32_t make_idesc_e4m3(int m, int n) {
 __host__ __device__ constexpr uint32_t make_idesc_nvf4(int m, int n) {
   return (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (0u << 23) |
          (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+// Instruction descriptor, kind::mxf4: e2m1 x e2m1, ue8m0 scales, K = 64. `half` picks the scale bytes of both operands: 0 the
+// first two of a row's four, 1 the last two.
+__host__ __device__ constexpr uint32_t make_idesc_mxf4(int m, int n, int half) {
+  return make_idesc_nvf4(m, n) | (1u << 23) | (static_cast<uint32_t>(half * 2) << 4) | (static_cast<uint32_t>(half * 2) << 29);
 }
 
 // ---------------------------------------------------------------- numeric helpers

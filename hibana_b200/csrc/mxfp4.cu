@@ -1,0 +1,223 @@
+// MXFP4 quantiser and its inverse for sm_100a.
+//
+// Format (OCP microscaling): blocks of 32 elements along K share a scale 2^(b - 127), b one byte (ue8m0); elements are e2m1.
+//   b = max(floor(log2(max |x|)) - 2 + 127, 0)      (2 = exponent of e2m1's largest value; zeros: b = 0)
+//   q = rne_e2m1(x * 2^(127 - b)), saturating at 6
+// A block that holds an infinity or a NaN gets b = 255, the format's NaN: what reads it returns NaN, not a clipped number.
+// The scale is a power of two, so x * 2^(127 - b) is exact and the only rounding is the one to e2m1.
+//
+// Packed values are row-major (low nibble first); scale bytes go to the 128 x 4 blocks that tcgen05.cp moves into TMEM, four
+// of a row (128 elements) being one 32-bit word.
+//
+// Bound by bytes: 2 (bf16) or 4 in and 17/32 out per element. Four lanes share a block: each holds eight elements (one or two
+// 16-byte loads), the maximum takes two shuffles, and sixteen lanes' scales make the word of an atom. A warp works on 1024
+// elements of a row at a time, all of its loads in flight at once.
+#include "hb_api.h"
+#include "hb_common.cuh"
+#include "rownorm.cuh"
+
+namespace hb {
+namespace {
+
+constexpr int QUANT_WARPS = 4;
+constexpr int SEG = 1024;              // elements of a row per warp: 4 steps of 256
+enum InType : int { kInBf16 = 0, kInF16 = 1, kInF32 = 2 };
+
+// Eight consecutive elements as floats; VEC: 16-byte aligned.
+template <int IN, bool VEC>
+struct Raw8 {
+  uint4 a, b;
+  __device__ __forceinline__ void load(const void* x, long long i) {
+    if constexpr (VEC) {
+      const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(x) + i * (IN == kInF32 ? 4 : 2));
+      a = ld_step(p);
+      if constexpr (IN == kInF32) b = ld_step(p + 1);
+    } else {
+      uint32_t w[8];
+      if constexpr (IN == kInF32) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = ld_step(static_cast<const uint32_t*>(x) + i + j);
+        b = make_uint4(w[4], w[5], w[6], w[7]);
+      } else {
+        const unsigned short* p = static_cast<const unsigned short*>(x) + i;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = static_cast<uint32_t>(ld_step(p + 2 * j)) | static_cast<uint32_t>(ld_step(p + 2 * j + 1)) << 16;
+      }
+      a = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+  __device__ __forceinline__ void floats(float (&f)[8]) const {
+    if constexpr (IN == kInBf16) {
+      unpack8(a, f);
+    } else if constexpr (IN == kInF16) {
+      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+        f[2 * j] = t.x;
+        f[2 * j + 1] = t.y;
+      }
+    } else {
+      const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(w[j]);
+    }
+  }
+};
+
+// src_rows (may be null; the expert-sorted buffers of a mixture-of-experts layer): rows with a negative entry are padding and
+// are left alone; with `gather` output row r takes input row src_rows[r]. Rows from *total_rows on are left alone too.
+template <int IN, bool VEC>
+__global__ void __launch_bounds__(QUANT_WARPS * 32)
+quant_mxfp4_kernel(const void* __restrict__ x, long long ldx, int m, int k, int ka, uint8_t* __restrict__ q,
+                   uint8_t* __restrict__ sf, int segs, const int* __restrict__ src_rows, const int* __restrict__ total_rows,
+                   int gather) {
+  grid_dep_wait(x, src_rows, total_rows);
+  grid_dep_launch();      // behind the wait: a grouped GEMM that follows reads the routing plan at once (see launch_dep)
+  const long long unit = static_cast<long long>(blockIdx.x) * QUANT_WARPS + (threadIdx.x >> 5);
+  const int row = static_cast<int>(unit / segs), seg = static_cast<int>(unit % segs), lane = threadIdx.x & 31;
+  if (row >= m || (total_rows != nullptr && row >= *total_rows)) return;
+  long long in_row = row;
+  if (src_rows != nullptr) {
+    const int s = src_rows[row];
+    if (s < 0) return;
+    if (gather) in_row = s;
+  }
+  const long long base = in_row * ldx;
+  const int k0 = seg * SEG + lane * 8;
+  Raw8<IN, VEC> raw[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (k0 + i * 256 < k) raw[i].load(x, base + k0 + i * 256);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = k0 + i * 256;                   // (k is a multiple of 32: a block is there as a whole or not at all)
+    if (seg * SEG + i * 256 >= ka * 128) break;   // uniform
+    float f[8];
+    uint32_t top = 0;
+    if (c < k) {
+      raw[i].floats(f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(f[j]) & 0x7FFFFFFFu);      // orders magnitudes, NaN last
+    }
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const uint32_t e = top >> 23;                 // 0: zero or below 2^-126, far under the smallest scale
+    const uint32_t b = e == 255u ? 255u : e > 2u ? e - 2u : 0u;
+    if (c < k) {
+      const float inv = __uint_as_float((b == 255u ? 127u : 254u - b) << 23);
+      uint32_t w = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w |= e2m1x2(f[2 * j] * inv, f[2 * j + 1] * inv) << (8 * j);
+      *reinterpret_cast<uint32_t*>(q + static_cast<size_t>(row) * (k >> 1) + (c >> 1)) = w;
+    }
+    // the four blocks of the 16 lanes' atom as one word; blocks that pad the last K tile have b = 0
+    uint32_t s = b << (8 * ((lane >> 2) & 3));
+    s |= __shfl_xor_sync(0xffffffffu, s, 4);
+    s |= __shfl_xor_sync(0xffffffffu, s, 8);
+    const int g = c >> 5;
+    if ((lane & 15) == 0 && (g >> 2) < ka) *reinterpret_cast<uint32_t*>(sf + row_sf_off(row, g, ka)) = s;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(void* out, size_t i, const float (&v)[8]);
+template <>
+__device__ __forceinline__ void store8<__nv_bfloat16>(void* out, size_t i, const float (&v)[8]) {
+  *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out) + i) = pack8(v);
+}
+template <>
+__device__ __forceinline__ void store8<__half>(void* out, size_t i, const float (&v)[8]) {
+  __half2 h[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) h[j] = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+  *reinterpret_cast<uint4*>(static_cast<__half*>(out) + i) = *reinterpret_cast<const uint4*>(h);
+}
+template <>
+__device__ __forceinline__ void store8<float>(void* out, size_t i, const float (&v)[8]) {
+  float4* p = reinterpret_cast<float4*>(static_cast<float*>(out) + i);
+  p[0] = make_float4(v[0], v[1], v[2], v[3]);
+  p[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+
+// Values of a packed matrix: e2m1 times 2^(b - 127). Both factors and (but for results past the largest float) the product are
+// exact in 32 bits; 16-bit outputs are rounded once. The same split of a row as above.
+template <typename T>
+__global__ void __launch_bounds__(QUANT_WARPS * 32)
+dequant_mxfp4_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ sf, int m, int k, int ka, void* __restrict__ out,
+                     int segs) {
+  grid_dep_wait(q, sf);
+  grid_dep_launch();
+  const long long unit = static_cast<long long>(blockIdx.x) * QUANT_WARPS + (threadIdx.x >> 5);
+  const int row = static_cast<int>(unit / segs), seg = static_cast<int>(unit % segs), lane = threadIdx.x & 31;
+  if (row >= m) return;
+  const int k0 = seg * SEG + lane * 8;
+  uint32_t w[4], b[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = k0 + i * 256;
+    if (c < k) {
+      w[i] = ld_step(reinterpret_cast<const uint32_t*>(q + static_cast<size_t>(row) * (k >> 1) + (c >> 1)));
+      b[i] = sf[row_sf_off(row, c >> 5, ka)];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = k0 + i * 256;
+    if (c >= k) break;
+    const float s = __uint_as_float(b[i] == 255u ? 0x7FC00000u : b[i] == 0u ? 0x00400000u : b[i] << 23);
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = e2m1_to_float((w[i] >> (4 * j)) & 15u) * s;
+    store8<T>(out, static_cast<size_t>(row) * k + c, v);
+  }
+}
+
+template <int IN>
+cudaError_t launch_quant(bool vec, const void* x, long long ldx, int m, int k, int ka, void* q, void* sf, const void* src_rows,
+                         const void* total_rows, int gather, cudaStream_t st) {
+  const int segs = (ka * 128 + SEG - 1) / SEG;
+  const long long units = static_cast<long long>(m) * segs, blocks = (units + QUANT_WARPS - 1) / QUANT_WARPS;
+  if (blocks > 0x7FFFFFFFll) return cudaErrorInvalidValue;
+  return launch_dep(vec ? quant_mxfp4_kernel<IN, true> : quant_mxfp4_kernel<IN, false>, dim3(static_cast<unsigned>(blocks)),
+                    dim3(QUANT_WARPS * 32), 0, st, x, ldx, m, k, ka, static_cast<uint8_t*>(q), static_cast<uint8_t*>(sf), segs,
+                    static_cast<const int*>(src_rows), static_cast<const int*>(total_rows), gather);
+}
+
+}  // namespace
+}  // namespace hb
+
+extern "C" {
+
+int hb_quant_mxfp4(const void* x, int in_type, long long ldx, int m, int k, int ka, void* q, void* sf, const void* src_rows,
+                   const void* total_rows, int gather, void* stream) {
+  using namespace hb;
+  if (m < 1 || k < 32 || k % 32 != 0 || ka != (k + 255) / 256 * 2) return 1;
+  const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ldx % (in_type == kInF32 ? 4 : 8) == 0;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  switch (in_type) {
+    case kInBf16: e = launch_quant<kInBf16>(vec, x, ldx, m, k, ka, q, sf, src_rows, total_rows, gather, st); break;
+    case kInF16: e = launch_quant<kInF16>(vec, x, ldx, m, k, ka, q, sf, src_rows, total_rows, gather, st); break;
+    case kInF32: e = launch_quant<kInF32>(vec, x, ldx, m, k, ka, q, sf, src_rows, total_rows, gather, st); break;
+    default: return 1;
+  }
+  return e == cudaSuccess ? 0 : 2;
+}
+
+int hb_dequant_mxfp4(const void* q, const void* sf, int m, int k, int ka, void* out, int out_type, void* stream) {
+  using namespace hb;
+  if (m < 1 || k < 32 || k % 32 != 0 || ka != (k + 255) / 256 * 2) return 1;
+  const int segs = (k + SEG - 1) / SEG;
+  const long long blocks = (static_cast<long long>(m) * segs + QUANT_WARPS - 1) / QUANT_WARPS;
+  if (blocks > 0x7FFFFFFFll) return 1;
+  auto kern = out_type == kInBf16 ? dequant_mxfp4_kernel<__nv_bfloat16> : out_type == kInF16 ? dequant_mxfp4_kernel<__half>
+                                                                                             : dequant_mxfp4_kernel<float>;
+  if (out_type < 0 || out_type > 2) return 1;
+  const cudaError_t e = launch_dep(kern, dim3(static_cast<unsigned>(blocks)), dim3(QUANT_WARPS * 32), 0,
+                                   static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(q),
+                                   static_cast<const uint8_t*>(sf), m, k, ka, out, segs);
+  return e == cudaSuccess ? 0 : 2;
+}
+
+}  // extern "C"

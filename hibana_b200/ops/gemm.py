@@ -1,4 +1,4 @@
-"""Linear layers on the tcgen05 GEMM (csrc/gemm.cu): bf16 and NVFP4, with fused epilogues.
+"""Linear layers on the tcgen05 GEMM (csrc/gemm.cu): bf16, NVFP4 and MXFP4, with fused epilogues.
 
 Dispatch: up to 256 tokens the weight matrix takes the 128-row MMA operand ("swap") and K is split across
 CTAs until the grid fills the 148 SMs, so a decode step streams every weight byte once at HBM rate; larger
@@ -14,6 +14,7 @@ import torch
 
 from .. import _native as nv
 from .. import config as cfgmod
+from .mxfp4 import Mxfp4Tensor
 from .nvfp4 import Nvfp4Tensor
 
 EPI_STORE, EPI_RESIDUAL, EPI_SILU_MUL, EPI_STORE_F32 = 0, 1, 2, 3
@@ -179,6 +180,48 @@ def linear_nvfp4(x: Nvfp4Tensor, w: Nvfp4Tensor, alpha: torch.Tensor, *, epilogu
     else:
         _launch(1, x.q, w.q, x.sf, w.sf, m, n, k, k, k, out, residual, 1.0, alpha, epilogue, False, splits, bn, x.ka,
                 w.ka)
+    return out
+
+
+def linear_mxfp4(x: Mxfp4Tensor, w: Mxfp4Tensor, *, epilogue: int = EPI_STORE, residual: Optional[torch.Tensor] = None,
+                 out: Optional[torch.Tensor] = None, splits: Optional[int] = None, static_weight: bool = False) -> torch.Tensor:
+    """y = dequant(x) @ dequant(w).T with block-scaled FP4 MMAs over the microscaled format (kind::mxf4), fp32 sums. Epilogues
+    as in `linear_nvfp4`; EPI_SILU_MUL takes interleaved gate / up rows (an even number) of `w`."""
+    m, k, n = x.rows, x.k, w.rows
+    if w.k != k:
+        raise ValueError(f"linear_mxfp4: x has K {k}, the weights have {w.k}")
+    if epilogue not in (EPI_STORE, EPI_RESIDUAL, EPI_SILU_MUL, EPI_STORE_F32) or (epilogue == EPI_SILU_MUL and n % 2):
+        raise ValueError(f"linear_mxfp4: epilogue {epilogue} does not fit {n} weight rows")
+    cols = n // 2 if epilogue == EPI_SILU_MUL else n
+    if (residual is not None) != (epilogue == EPI_RESIDUAL) or (residual is not None and (
+            residual.shape != (m, cols) or residual.dtype != torch.bfloat16)):
+        raise ValueError("linear_mxfp4: the residual epilogue, and no other, takes a bf16 residual of the output's shape")
+    if x.q.device != w.q.device or (residual is not None and residual.device != x.q.device):
+        raise ValueError("linear_mxfp4: operands on different devices")
+    if not nv.use_native(x.q, w.q):
+        acc = x.dequantize() @ w.dequantize().t()
+        res = _ref_epilogue(acc, epilogue, residual)
+        if out is not None:
+            out.copy_(res)
+            return out
+        return res
+    out = _out(m, n, epilogue, x.q, out)
+    if out.device != x.q.device or out.data_ptr() % 16:
+        raise ValueError("linear_mxfp4: the output must be on the operands' device and start on a 16-byte boundary")
+    if m == 0:
+        return out
+    if residual is not None and (residual.stride() != out.stride() or residual.data_ptr() % 16):
+        # the epilogue reads it where it writes the output
+        residual = torch.empty_strided(out.shape, out.stride(), dtype=out.dtype, device=out.device).copy_(residual)
+    with nv.on_device(x.q):
+        if not static_weight:
+            nv.lib().hb_gemm_plain()
+        swap, bn, auto_splits = _plan(m, n, (k + 255) // 256, nv.WORKSPACE_BYTES)
+        splits = auto_splits if splits is None else splits
+        if swap:
+            _launch(4, w.q, x.q, w.sf, x.sf, n, m, k, k, k, out, residual, 1.0, None, epilogue, True, splits, bn, w.ka, x.ka)
+        else:
+            _launch(4, x.q, w.q, x.sf, w.sf, m, n, k, k, k, out, residual, 1.0, None, epilogue, False, splits, bn, x.ka, w.ka)
     return out
 
 

@@ -52,8 +52,12 @@ def from_e4m3(b: torch.Tensor) -> torch.Tensor:
 
 def swizzle_sf(sf: torch.Tensor) -> torch.Tensor:
     """[rows, K/16] uint8 row-major scales -> [ceil(rows/128), k_atoms, 512] swizzled blocks (zero padded)."""
+    return swizzle_blocks(sf, k_atoms(sf.shape[1] * 16))
+
+
+def swizzle_blocks(sf: torch.Tensor, ka: int) -> torch.Tensor:
+    """[rows, groups] uint8 row-major scales -> [ceil(rows/128), ka, 512] swizzled blocks (zero padded)."""
     rows, groups = sf.shape
-    ka = k_atoms(groups * 16)
     rb = (rows + 127) // 128
     rb += rb & 1 if rb > 1 else 0  # whole 256-row tiles, so a 128 x 256 MMA tile never reads past the end
     full = torch.zeros(rb * 128, ka * 4, dtype=torch.uint8, device=sf.device)
