@@ -565,6 +565,17 @@ __device__ __forceinline__ uint32_t e2m1x2(float lo, float hi) {
       : "f"(hi), "f"(lo));
   return r;
 }
+// One byte of e2m1 codes -> two fp16 numbers (exact), low nibble in the low half; and as floats.
+__device__ __forceinline__ uint32_t e2m1x2_to_half2(uint32_t byte) {
+  uint32_t h2;
+  const uint16_t in = static_cast<uint16_t>(byte);
+  asm("{\n\t.reg .b8 t;\n\tcvt.u8.u16 t, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, t;\n\t}" : "=r"(h2) : "h"(in));
+  return h2;
+}
+__device__ __forceinline__ float2 e2m1x2_to_float2(uint32_t byte) {
+  const uint32_t h2 = e2m1x2_to_half2(byte);
+  return __half22float2(*reinterpret_cast<const __half2*>(&h2));
+}
 __device__ __forceinline__ float e2m1_to_float(uint32_t c) {
   const float t[8] = {0.f, .5f, 1.f, 1.5f, 2.f, 3.f, 4.f, 6.f};
   const float v = t[c & 7];

@@ -74,8 +74,9 @@ quant_mxfp4_kernel(const void* __restrict__ x, long long ldx, int m, int k, int 
                    int gather) {
   grid_dep_wait(x, src_rows, total_rows);
   grid_dep_launch();      // behind the wait: a grouped GEMM that follows reads the routing plan at once (see launch_dep)
-  const long long unit = static_cast<long long>(blockIdx.x) * QUANT_WARPS + (threadIdx.x >> 5);
-  const int row = static_cast<int>(unit / segs), seg = static_cast<int>(unit % segs), lane = threadIdx.x & 31;
+  const uint32_t unit = blockIdx.x * QUANT_WARPS + (threadIdx.x >> 5);      // (the launch keeps it below 2^31)
+  const int row = static_cast<int>(unit / static_cast<uint32_t>(segs)), seg = static_cast<int>(unit) - row * segs;
+  const int lane = threadIdx.x & 31;
   if (row >= m || (total_rows != nullptr && row >= *total_rows)) return;
   long long in_row = row;
   if (src_rows != nullptr) {
@@ -148,8 +149,9 @@ dequant_mxfp4_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ 
                      int segs) {
   grid_dep_wait(q, sf);
   grid_dep_launch();
-  const long long unit = static_cast<long long>(blockIdx.x) * QUANT_WARPS + (threadIdx.x >> 5);
-  const int row = static_cast<int>(unit / segs), seg = static_cast<int>(unit % segs), lane = threadIdx.x & 31;
+  const uint32_t unit = blockIdx.x * QUANT_WARPS + (threadIdx.x >> 5);      // (the launch keeps it below 2^31)
+  const int row = static_cast<int>(unit / static_cast<uint32_t>(segs)), seg = static_cast<int>(unit) - row * segs;
+  const int lane = threadIdx.x & 31;
   if (row >= m) return;
   const int k0 = seg * SEG + lane * 8;
   uint32_t w[4], b[4];
@@ -168,7 +170,11 @@ dequant_mxfp4_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ 
     const float s = __uint_as_float(b[i] == 255u ? 0x7FC00000u : b[i] == 0u ? 0x00400000u : b[i] << 23);
     float v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = e2m1_to_float((w[i] >> (4 * j)) & 15u) * s;
+    for (int j = 0; j < 4; ++j) {
+      const float2 t = e2m1x2_to_float2((w[i] >> (8 * j)) & 255u);
+      v[2 * j] = t.x * s;
+      v[2 * j + 1] = t.y * s;
+    }
     store8<T>(out, static_cast<size_t>(row) * k + c, v);
   }
 }
@@ -178,7 +184,7 @@ cudaError_t launch_quant(bool vec, const void* x, long long ldx, int m, int k, i
                          const void* total_rows, int gather, cudaStream_t st) {
   const int segs = (ka * 128 + SEG - 1) / SEG;
   const long long units = static_cast<long long>(m) * segs, blocks = (units + QUANT_WARPS - 1) / QUANT_WARPS;
-  if (blocks > 0x7FFFFFFFll) return cudaErrorInvalidValue;
+  if (units > 0x7FFFFFF0ll) return cudaErrorInvalidValue;
   return launch_dep(vec ? quant_mxfp4_kernel<IN, true> : quant_mxfp4_kernel<IN, false>, dim3(static_cast<unsigned>(blocks)),
                     dim3(QUANT_WARPS * 32), 0, st, x, ldx, m, k, ka, static_cast<uint8_t*>(q), static_cast<uint8_t*>(sf), segs,
                     static_cast<const int*>(src_rows), static_cast<const int*>(total_rows), gather);
@@ -210,7 +216,7 @@ int hb_dequant_mxfp4(const void* q, const void* sf, int m, int k, int ka, void* 
   if (m < 1 || k < 32 || k % 32 != 0 || ka != (k + 255) / 256 * 2) return 1;
   const int segs = (k + SEG - 1) / SEG;
   const long long blocks = (static_cast<long long>(m) * segs + QUANT_WARPS - 1) / QUANT_WARPS;
-  if (blocks > 0x7FFFFFFFll) return 1;
+  if (static_cast<long long>(m) * segs > 0x7FFFFFF0ll) return 1;
   auto kern = out_type == kInBf16 ? dequant_mxfp4_kernel<__nv_bfloat16> : out_type == kInF16 ? dequant_mxfp4_kernel<__half>
                                                                                              : dequant_mxfp4_kernel<float>;
   if (out_type < 0 || out_type > 2) return 1;

@@ -16,7 +16,7 @@ import torch
 import torch.nn.functional as F
 
 from .. import _native as nv
-from . import gemm, nvfp4
+from . import gemm, mxfp4, nvfp4
 
 P, I, L, Fl = nv.P, nv.I, nv.L, nv.F
 nv.register("hb_moe_route", [P, L, P, I, I, I, I, I, Fl, P, P, P])
@@ -126,12 +126,13 @@ def share_experts(ids: torch.Tensor, weights: torch.Tensor, experts: int, keep: 
 @dataclass
 class ExpertWeights:
     """Stacked expert matrices. fc1: [E * n1, H] rows (n1 = 2I interleaved for SwiGLU, I for ReLU^2); fc2:
-    [E * H_out, I]. For NVFP4 `*_q` are Nvfp4Tensors over the stacked rows and `*_alpha` [E] = act_scale * w_scale."""
+    [E * H_out, I]. For NVFP4 `*_q` are Nvfp4Tensors over the stacked rows and `*_alpha` [E] = act_scale * w_scale; for MXFP4
+    they are Mxfp4Tensors and there is nothing else."""
     experts: int
     hidden: int           # input width of fc1 / output width of fc2
     inter: int
     act: str              # swiglu | relu2
-    fmt: str              # bf16 | nvfp4
+    fmt: str              # bf16 | nvfp4 | mxfp4 | w3
     fc1: object
     fc2: object
     fc1_alpha: Optional[torch.Tensor] = None
@@ -153,6 +154,9 @@ class ExpertWeights:
             return cls(e, h, inter, act, fmt, fc1.reshape(e * n1, h).to(torch.bfloat16).contiguous(),
                        fc2.reshape(e * fc2.shape[1], inter).to(torch.bfloat16).contiguous())
         dev = fc1.device
+        if fmt == "mxfp4":
+            return cls(e, h, inter, act, fmt, mxfp4.quantize_weight(fc1.reshape(e * n1, h)),
+                       mxfp4.quantize_weight(fc2.reshape(e * fc2.shape[1], inter)))
         if fmt == "w3":
             # 3-bit experts (groups of 64, scale + zero): one tile stack over all experts' rows; an expert's rows
             # are a multiple of 128, so expert boundaries fall on tile boundaries
@@ -194,6 +198,8 @@ class ExpertWeights:
             return self.w3[which - 1].dequantize().view(self.experts, n, -1).to(w.device)
         if self.fmt == "bf16":
             return w.float().view(self.experts, n, -1)
+        if self.fmt == "mxfp4":
+            return w.dequantize().view(self.experts, n, -1)
         sfb = nvfp4.unswizzle_sf(w.sf, w.rows, w.k // 16)
         out = torch.empty(w.rows, w.k, dtype=torch.float32, device=w.q.device)
         for e in range(self.experts):
@@ -215,10 +221,12 @@ class ExpertWeights:
             if self.fmt == "bf16":
                 return w[e_lo * n:(e_lo + e_n) * n]
             assert n % 128 == 0, "scale blocks cover 128 rows: expert boundaries must fall on them"
+            if self.fmt == "mxfp4":
+                return mxfp4.Mxfp4Tensor(w.q[e_lo * n:(e_lo + e_n) * n], w.sf[e_lo * n // 128:(e_lo + e_n) * n // 128], e_n * n, w.k)
             return nvfp4.Nvfp4Tensor(w.q[e_lo * n:(e_lo + e_n) * n], w.sf[e_lo * n // 128:(e_lo + e_n) * n // 128],
                                      w.gscale[e_lo:e_lo + e_n], e_n * n, w.k)
 
-        cut = (lambda v: v[e_lo:e_lo + e_n].contiguous()) if self.fmt != "bf16" else (lambda v: v)
+        cut = (lambda v: v[e_lo:e_lo + e_n].contiguous()) if self.fmt == "nvfp4" else (lambda v: v)
         return ExpertWeights(e_n, self.hidden, self.inter, self.act, self.fmt, rows(self.fc1, n1), rows(self.fc2, n2),
                              cut(self.fc1_alpha), cut(self.fc2_alpha), self.fc1_in_scale, self.fc2_in_scale)
 
@@ -226,6 +234,8 @@ class ExpertWeights:
         def mv(x):
             if isinstance(x, nvfp4.Nvfp4Tensor):
                 return nvfp4.Nvfp4Tensor(x.q.to(device), x.sf.to(device), x.gscale.to(device), x.rows, x.k)
+            if isinstance(x, mxfp4.Mxfp4Tensor):
+                return x.to(device)
             return x.to(device) if isinstance(x, torch.Tensor) else x
         out = ExpertWeights(self.experts, self.hidden, self.inter, self.act, self.fmt, mv(self.fc1), mv(self.fc2),
                             mv(self.fc1_alpha), mv(self.fc2_alpha), mv(self.fc1_in_scale), mv(self.fc2_in_scale))
@@ -251,6 +261,8 @@ def experts_ref(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, ew: E
     if ew.fmt == "nvfp4":   # same activation quantisation as the kernel path
         q, sfb = nvfp4.quantize_ref(x, ew.fc1_in_scale)
         xf = nvfp4.dequantize_ref(q, sfb, ew.fc1_in_scale)
+    elif ew.fmt == "mxfp4":
+        xf = mxfp4.dequantize_ref(*mxfp4.quantize_ref(x))
     out = torch.zeros(t, ew.fc2_rows, dtype=torch.float32, device=x.device)
     for ti in range(t):
         for k in range(ids.shape[1]):
@@ -262,6 +274,8 @@ def experts_ref(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, ew: E
             if ew.fmt == "nvfp4":
                 q, sfb = nvfp4.quantize_ref(mid.view(1, -1), ew.fc2_in_scale)
                 midf = nvfp4.dequantize_ref(q, sfb, ew.fc2_in_scale)[0]
+            elif ew.fmt == "mxfp4":
+                midf = mxfp4.dequantize_ref(*mxfp4.quantize_ref(mid.view(1, -1)))[0]
             else:
                 midf = mid.float()
             y = (midf @ w2[e].t()).to(torch.bfloat16).float()
@@ -279,7 +293,7 @@ def tile_hint(pairs: int, experts: int, max_rows: int, fmt: str) -> int:
     bn = 16
     while bn < min(avg + avg // 4, 128):     # 128 at most: up to that width two CTAs share an SM (csrc/gemm.cu Cfg)
         bn *= 2
-    if fmt == "nvfp4" and bn < 128 and max_rows > bn:
+    if fmt in ("nvfp4", "mxfp4") and bn < 128 and max_rows > bn:
         bn = 128
     return bn
 
@@ -348,6 +362,16 @@ def experts_forward(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, e
         nv.check(lib.hb_gemm_grouped(kind, ew.fc2.data_ptr(), mid.data_ptr(), None, None, e, h_out, rows_cap,
                                      ew.inter, y.data_ptr(), y.stride(0), None, gemm.EPI_STORE, start.data_ptr(),
                                      cnt.data_ptr(), max_rows, st.data_ptr(), 0, 0, bn_hint, *tl, nv.stream()), "hb_gemm_grouped")
+    elif ew.fmt == "mxfp4":
+        q1 = mxfp4.quantize(x, src_rows=src, total_rows=total, rows=rows_cap, gather=True)
+        nv.check(lib.hb_gemm_grouped(4, ew.fc1.q.data_ptr(), q1.q.data_ptr(), ew.fc1.sf.data_ptr(), q1.sf.data_ptr(), e, n1,
+                                     rows_cap, h, h1.data_ptr(), h1.stride(0), None, epi1, start.data_ptr(), cnt.data_ptr(),
+                                     max_rows, st.data_ptr(), ew.fc1.ka, q1.ka, bn_hint, *tl, nv.stream()), "hb_gemm_grouped")
+        q2 = mxfp4.quantize(h1, src_rows=src, total_rows=total)      # (the padding between segments stays as it is)
+        nv.check(lib.hb_gemm_grouped(4, ew.fc2.q.data_ptr(), q2.q.data_ptr(), ew.fc2.sf.data_ptr(), q2.sf.data_ptr(), e, h_out,
+                                     rows_cap, ew.inter, y.data_ptr(), y.stride(0), None, gemm.EPI_STORE, start.data_ptr(),
+                                     cnt.data_ptr(), max_rows, st.data_ptr(), ew.fc2.ka, q2.ka, bn_hint, *tl, nv.stream()),
+                 "hb_gemm_grouped")
     else:
         q1, sf1 = nvfp4._alloc(rows_cap, h, dev)
         # few pairs (decode, verify): quantise by pair, not by row of the padded buffer (most of which is padding
@@ -392,3 +416,113 @@ def experts_forward(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, e
                                 shared.stride(0) if shared is not None else 0, out.data_ptr(), out.stride(0), t, topk,
                                 h_out, nv.stream()), "hb_moe_combine")
     return out
+
+
+FEW_TOKENS = 16          # tokens up to which a layer runs in two kernels (csrc/moe_few.cu)
+_KINDS = {"bf16": 0, "nvfp4": 1, "mxfp4": 4}
+
+nv.register("hb_moe_few_tokens", [I, I, I, I])
+nv.register("hb_moe_few", [I, P, L, P, L, P, L, I, P, L, P, I, I, I, I, I, Fl, I, I, I, I, P, P, P, I, P, P, P, I, P, L, P, L, P, I, I,
+                           P])
+
+
+def few_tokens_ref(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, ew: ExpertWeights,
+                   shared: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Plain PyTorch of the few-token form: activations are not quantised, nothing is rounded before the end."""
+    w1, w2 = ew.dense(1), ew.dense(2)
+    out = torch.zeros(x.shape[0], ew.fc2_rows, dtype=torch.float32, device=x.device)
+    for t in range(x.shape[0]):
+        for j in range(ids.shape[1]):
+            e = int(ids[t, j])
+            out[t] += weights[t, j] * (_act(x[t].float() @ w1[e].t(), ew.act) @ w2[e].t())
+    return (out if shared is None else out + shared.float()).to(torch.bfloat16)
+
+
+def few_tokens_ok(ew: ExpertWeights, topk: int) -> bool:
+    """Whether the two-kernel form covers a layer: bf16, NVFP4 or MXFP4 experts, at most 1024 of them and 32 a token, with
+    whole tiles (128 rows of FP4 weights and their scales, 16 rows in bf16) per expert and matrix."""
+    rows, k = (16, 8) if ew.fmt == "bf16" else (128, 32)
+    return (ew.fmt in _KINDS and ew.act in ("swiglu", "relu2") and ew.experts <= 1024 and topk <= 32 and ew.n1 % rows == 0
+            and ew.fc2_rows % rows == 0 and ew.hidden % k == 0 and ew.inter % k == 0)
+
+
+def _rows16(x: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """Rows that 16-byte loads can read: as they are, or copied."""
+    if x is None or (x.stride(-1) == 1 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0):
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
+def layer_forward(x: torch.Tensor, router: torch.Tensor, ew: ExpertWeights, topk: int, *, sigmoid: bool = False,
+                  sel_bias: Optional[torch.Tensor] = None, renorm: bool = True, scale: float = 1.0,
+                  shared: Optional[torch.Tensor] = None, route_x: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A whole mixture-of-experts layer: x [T, H] bf16 -> [T, H_out] bf16.
+
+    router bf16 [E, Hr]; its input rows are `route_x` [T, Hr] (a latent layer routes on the hidden rows) or x. Scores, top-k and
+    weights as in `route`; `shared` [T, H_out] bf16 is added to the sum. Up to FEW_TOKENS tokens the layer is two kernels
+    that stream the chosen experts' weights once and read the activations in bf16, whatever the experts' format; more
+    tokens, and layers `few_tokens_ok` does not cover, take `linear_bf16`, `route` and `experts_forward` (which quantises
+    activations for FP4 experts)."""
+    if x.dim() != 2 or x.dtype != torch.bfloat16 or x.shape[1] != ew.hidden:
+        raise ValueError(f"layer_forward: bf16 rows of width {ew.hidden} expected, got {x.dtype} {tuple(x.shape)}")
+    t, e = x.shape[0], ew.experts
+    rx = x if route_x is None else route_x
+    if router.dim() != 2 or router.shape[0] != e or router.dtype != torch.bfloat16:
+        raise ValueError(f"layer_forward: a bf16 router of {e} rows expected, got {router.dtype} {tuple(router.shape)}")
+    if rx.shape != (t, router.shape[1]) or rx.dtype != torch.bfloat16:
+        raise ValueError(f"layer_forward: bf16 router input {(t, router.shape[1])} expected, got {rx.dtype} {tuple(rx.shape)}")
+    if not 1 <= topk <= e:
+        raise ValueError(f"layer_forward: top-{topk} of {e} experts")
+    if sel_bias is not None and (not sigmoid or sel_bias.shape != (e,) or sel_bias.dtype != torch.float32):
+        raise ValueError("layer_forward: the selection bias is fp32, one number an expert, and goes with sigmoid scores")
+    if shared is not None and (shared.shape != (t, ew.fc2_rows) or shared.dtype != torch.bfloat16):
+        raise ValueError(f"layer_forward: bf16 shared rows {(t, ew.fc2_rows)} expected, got {shared.dtype} {tuple(shared.shape)}")
+    w1 = ew.fc1 if isinstance(ew.fc1, torch.Tensor) else ew.fc1.q
+    for other in (router, rx, w1, sel_bias, shared):
+        if other is not None and other.device != x.device:
+            raise ValueError("layer_forward: operands on different devices")
+    few = t <= FEW_TOKENS and few_tokens_ok(ew, topk)
+    route_args = {"sigmoid": sigmoid, "sel_bias": sel_bias, "renorm": renorm, "scale": scale}
+    if not nv.use_native(x):
+        ids, w = route_ref(rx.float() @ router.float().t(), topk, **route_args)
+        return few_tokens_ref(x, ids, w, ew, shared) if few else experts_forward(x, ids, w, ew, shared=shared)
+    with nv.on_device(x):
+        if t == 0:
+            return torch.empty(0, ew.fc2_rows, dtype=torch.bfloat16, device=x.device)
+        kind = _KINDS.get(ew.fmt, 0)
+        most = nv.lib().hb_moe_few_tokens(kind, ew.hidden, e, FC1_CLUSTER) if few else 0
+        if most == 0 or router.shape[1] % 8:
+            ids, w = route(gemm.linear_bf16(rx, router, epilogue=gemm.EPI_STORE_F32), topk, **route_args)
+            return experts_forward(x, ids, w, ew, shared=shared)
+        out = torch.empty(t, ew.fc2_rows, dtype=torch.bfloat16, device=x.device)
+        x, rx, router, shared = _rows16(x), _rows16(rx), _rows16(router), _rows16(shared)
+        if sel_bias is not None:
+            sel_bias = sel_bias.contiguous()
+        for lo in range(0, t, most):
+            _few_launch(kind, x[lo:lo + most], rx[lo:lo + most], router, ew, topk, route_args, sel_bias,
+                        None if shared is None else shared[lo:lo + most], out[lo:lo + most])
+    return out
+
+
+FC1_CLUSTER = 8
+
+
+def _fc2_cluster(rows: int) -> int:
+    """CTAs that share the experts of a 16-row tile of the output, so that the tiles fill two CTAs an SM."""
+    return max(1, min(8, 2 * gemm.NUM_SMS // (rows // 16)))
+
+
+def _few_launch(kind, x, rx, router, ew, topk, ra, sel_bias, shared, out) -> None:
+    t = x.shape[0]
+    pairs = -(-(t * topk) // 16) * 16
+    ws = torch.empty(pairs * (8 + 4 * ew.inter + -(-(ew.inter // 8) // 16) * 16), dtype=torch.uint8, device=x.device)
+    if kind == 0:
+        w1, w2 = (ew.fc1.data_ptr(), None, None, 0), (ew.fc2.data_ptr(), None, None, 0)
+    else:
+        w1, w2 = ((w.q.data_ptr(), w.sf.data_ptr(), w.gscale.data_ptr() if kind == 1 else None, w.ka) for w in (ew.fc1, ew.fc2))
+    nv.check(nv.lib().hb_moe_few(kind, x.data_ptr(), x.stride(0), rx.data_ptr(), rx.stride(0), router.data_ptr(), router.stride(0),
+                                 router.shape[1], None, 0, nv.ptr(sel_bias), t, ew.experts, topk, int(ra["sigmoid"]),
+                                 int(ra["renorm"]), ra["scale"], ew.hidden, ew.inter, ew.fc2_rows, int(ew.act == "swiglu"), *w1,
+                                 *w2, nv.ptr(shared), shared.stride(0) if shared is not None else 0, out.data_ptr(),
+                                 out.stride(0), ws.data_ptr(), FC1_CLUSTER, _fc2_cluster(ew.fc2_rows), nv.stream()),
+             "hb_moe_few", launches=2)
