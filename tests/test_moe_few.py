@@ -198,7 +198,7 @@ def test_strided_rows_wide_layers_and_outputs_gpu(fmt):
         wide = lambda v: torch.zeros(v.shape[0], width, dtype=v.dtype, device="cuda")[:, lead:lead + 256].copy_(v)   # noqa: E731
         assert torch.equal(moe.layer_forward(wide(x), wide(router), ewg, 2, shared=wide(sh)), want)
     ew, x, rx, router, bias, sh = _case(16, 4, 8192, "relu2", fmt, 128, h_out=128, std=0.02)
-    assert nv.lib().hb_moe_few_tokens(moe._KINDS[fmt], 8192, 4, moe.FC1_CLUSTER) < 16
+    assert nv.lib().hb_moe_few_tokens(moe._KINDS[fmt], 8192, 128, 4, moe.FC1_CLUSTER) < 16
     got = moe.layer_forward(x.cuda(), router.cuda(), ew.to("cuda"), 2, shared=sh.cuda())
     _check(got, *_exact(ew, x, None, router, 2, False, bias, 1.0, sh))
 
