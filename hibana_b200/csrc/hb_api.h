@@ -265,16 +265,15 @@ int hb_moe_gather(const void* x, long long ldx, const void* src_row, const void*
 int hb_moe_combine(const void* y, long long ldy, const void* pos, const void* weights, const void* shared,
                    long long ld_shared, void* out, long long ldo, int tokens, int topk, int h, void* stream);
 
-// A whole mixture-of-experts layer of up to hb_moe_few_tokens(...) tokens in two kernels (moe_few.cu). kind: format of the experts
-// (0 bf16, 1 nvfp4 with gs1 / gs2 one scale per expert, 4 mxfp4). route_x null: the router reads x. ws: workspace of
-// (8 + 4 * inter) bytes for each of the tokens * topk pairs, rounded up to 16. cluster1: CTAs per cluster of the first kernel;
-// row_tiles, cluster2: 16-row tiles per CTA and CTAs per cluster of the second.
-int hb_moe_few_tokens(int kind, int hidden, int inter, int experts, int cluster);
+// A mixture-of-experts layer of up to hb_moe_few_tokens(...) tokens: router, fc1, fc2 (moe_few.cu). kind: format of the experts
+// (0 bf16, 1 nvfp4 with gs1 / gs2 one scale per expert, 4 mxfp4). ws: hb_moe_few_ws(...) bytes, 128-byte aligned.
+int hb_moe_few_tokens(int kind, int hidden);
+int hb_moe_few_ws(int kind, int tokens, int experts, int topk, int hidden, int inter);
 int hb_moe_few(int kind, const void* x, long long ldx, const void* route_x, long long ld_route, const void* router,
                long long ld_router, int route_k, const void* sel_bias, int tokens, int experts, int topk, int sigmoid, int renorm,
                float scale, int hidden, int inter, int h_out, int swiglu, const void* w1, const void* sf1, const void* gs1, int ka1,
                const void* w2, const void* sf2, const void* gs2, int ka2, const void* shared, long long ld_shared, void* out,
-               long long ldo, void* ws, int cluster1, int row_tiles, int cluster2, void* stream);
+               long long ldo, void* ws, void* status, void* stream);
 
 #ifdef __cplusplus
 }

@@ -9,7 +9,6 @@ hibana/kernels/w3_moe.py:194 (reference), hibana/kernels/csrc/w3_gemm.cu:640-130
 """
 from __future__ import annotations
 
-import functools
 from dataclasses import dataclass
 from typing import Optional
 
@@ -419,11 +418,12 @@ def experts_forward(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, e
     return out
 
 
-FEW_TOKENS = 16          # tokens up to which a layer runs in two kernels (csrc/moe_few.cu)
+FEW_TOKENS = 16          # tokens up to which a layer runs in csrc/moe_few.cu
 _KINDS = {"bf16": 0, "nvfp4": 1, "mxfp4": 4}
 
-nv.register("hb_moe_few_tokens", [I, I, I, I, I])
-nv.register("hb_moe_few", [I, P, L, P, L, P, L, I, P, I, I, I, I, I, Fl, I, I, I, I, P, P, P, I, P, P, P, I, P, L, P, L, P, I, I, I, P])
+nv.register("hb_moe_few_tokens", [I, I])
+nv.register("hb_moe_few_ws", [I, I, I, I, I, I])
+nv.register("hb_moe_few", [I, P, L, P, L, P, L, I, P, I, I, I, I, I, Fl, I, I, I, I, P, P, P, I, P, P, P, I, P, L, P, L, P, P, P])
 
 
 def few_tokens_ref(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, ew: ExpertWeights,
@@ -440,8 +440,8 @@ def few_tokens_ref(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, ew
 
 def few_tokens_ok(ew: ExpertWeights, topk: int) -> bool:
     """Whether the two-kernel form covers a layer: bf16, NVFP4 or MXFP4 experts, at most 1024 of them and 32 a token, with
-    whole tiles (128 rows of FP4 weights and their scales, 16 rows in bf16) per expert and matrix."""
-    rows, k = (16, 8) if ew.fmt == "bf16" else (128, 32)
+    whole blocks (128 rows of FP4 weights and their scales) per expert and matrix."""
+    rows, k = (8, 8) if ew.fmt == "bf16" else (128, 32)
     return (ew.fmt in _KINDS and ew.act in ("swiglu", "relu2") and ew.experts <= 1024 and topk <= 32 and ew.n1 % rows == 0
             and ew.fc2_rows % rows == 0 and ew.hidden % k == 0 and ew.inter % k == 0)
 
@@ -490,47 +490,30 @@ def layer_forward(x: torch.Tensor, router: torch.Tensor, ew: ExpertWeights, topk
         if t == 0:
             return torch.empty(0, ew.fc2_rows, dtype=torch.bfloat16, device=x.device)
         kind = _KINDS.get(ew.fmt, 0)
-        most = nv.lib().hb_moe_few_tokens(kind, ew.hidden, ew.inter, e, FC1_CLUSTER) if few else 0
-        if most == 0 or router.shape[1] % 8:
+        most = nv.lib().hb_moe_few_tokens(kind, ew.hidden) if few else 0       # (a wide layer's rows take several calls)
+        if most * 2 < t or router.shape[1] % 8:
             ids, w = route(gemm.linear_bf16(rx, router, epilogue=gemm.EPI_STORE_F32), topk, **route_args)
             return experts_forward(x, ids, w, ew, shared=shared)
         out = torch.empty(t, ew.fc2_rows, dtype=torch.bfloat16, device=x.device)
         x, router, shared = _rows16(x), _rows16(router), _rows16(shared)
-        rx = None if route_x is None else _rows16(route_x)
+        rx = x if route_x is None else _rows16(route_x)
         if sel_bias is not None:
             sel_bias = sel_bias.contiguous()
         for lo in range(0, t, most):
-            _few_launch(kind, x[lo:lo + most], None if rx is None else rx[lo:lo + most], router, ew, topk, route_args, sel_bias,
+            _few_launch(kind, x[lo:lo + most], rx[lo:lo + most], router, ew, topk, route_args, sel_bias,
                         None if shared is None else shared[lo:lo + most], out[lo:lo + most])
     return out
 
 
-FC1_CLUSTER = 16         # CTAs that compute the routing together (each cluster computes all of it)
-
-
-@functools.lru_cache(maxsize=256)
-def _fc2_grid(rows: int) -> tuple[int, int]:
-    """(16-row tiles a CTA, CTAs a cluster) of the second kernel: the pair that keeps most SMs busy, of those the one with most
-    tiles a CTA (its rows of mid are converted once for all of them). The CTAs of a cluster share the experts."""
-    tiles, best = rows // 16, (0.0, 0, 0)
-    for per in (1, 2, 4, 8, 16):
-        blocks = -(-tiles // per)
-        cluster = max(1, min(8, gemm.NUM_SMS // blocks))
-        waves = -(-blocks * cluster // gemm.NUM_SMS)
-        best = max(best, (tiles * cluster / (per * waves), per, cluster))
-    return best[1], best[2]
-
-
 def _few_launch(kind, x, rx, router, ew, topk, ra, sel_bias, shared, out) -> None:
-    t = x.shape[0]
-    ws = torch.empty(-(-(t * topk) // 16) * 16 * (8 + 4 * ew.inter), dtype=torch.uint8, device=x.device)
+    t, lib = x.shape[0], nv.lib()
+    ws = torch.empty(lib.hb_moe_few_ws(kind, t, ew.experts, topk, ew.hidden, ew.inter), dtype=torch.uint8, device=x.device)
     if kind == 0:
         w1, w2 = (ew.fc1.data_ptr(), None, None, 0), (ew.fc2.data_ptr(), None, None, 0)
     else:
         w1, w2 = ((w.q.data_ptr(), w.sf.data_ptr(), w.gscale.data_ptr() if kind == 1 else None, w.ka) for w in (ew.fc1, ew.fc2))
-    nv.check(nv.lib().hb_moe_few(kind, x.data_ptr(), x.stride(0), nv.ptr(rx), 0 if rx is None else rx.stride(0),
-                                 router.data_ptr(), router.stride(0), router.shape[1], nv.ptr(sel_bias), t, ew.experts, topk,
-                                 int(ra["sigmoid"]), int(ra["renorm"]), ra["scale"], ew.hidden, ew.inter, ew.fc2_rows,
-                                 int(ew.act == "swiglu"), *w1, *w2, nv.ptr(shared), shared.stride(0) if shared is not None else 0,
-                                 out.data_ptr(), out.stride(0), ws.data_ptr(), FC1_CLUSTER, *_fc2_grid(ew.fc2_rows), nv.stream()),
-             "hb_moe_few", launches=2)
+    nv.check(lib.hb_moe_few(kind, x.data_ptr(), x.stride(0), rx.data_ptr(), rx.stride(0), router.data_ptr(), router.stride(0),
+                            router.shape[1], nv.ptr(sel_bias), t, ew.experts, topk, int(ra["sigmoid"]), int(ra["renorm"]),
+                            ra["scale"], ew.hidden, ew.inter, ew.fc2_rows, int(ew.act == "swiglu"), *w1, *w2, nv.ptr(shared),
+                            shared.stride(0) if shared is not None else 0, out.data_ptr(), out.stride(0), ws.data_ptr(),
+                            nv.device_state(x.device).status.data_ptr(), nv.stream()), "hb_moe_few", launches=3)

@@ -36,14 +36,17 @@ def _exact(ew, x, rx, router, topk, sigmoid, bias, scale, shared, renorm=True):
     w1, w2 = ew.dense(1).double(), ew.dense(2).double()
     out = torch.zeros(x.shape[0], ew.fc2_rows, dtype=torch.float64)
     err = torch.zeros_like(out)
-    # sums of n terms in 32 bits: n * 2^-23 of what is added up in magnitude; mid keeps 11 bits (8 for bf16 experts); exponentials,
+    # sums of n terms in 32 bits: n * 2^-23 of what is added up in magnitude; x and mid keep 14 bits of
+    # their block's largest number, counted here from the row's (bf16 experts: x all, mid 16 bits); exponentials,
     # quotients and weights within 2^-18
-    mid_half = 2.0 ** -9 if ew.fmt == "bf16" else 2.0 ** -12
+    digits = 0.0 if ew.fmt == "bf16" else 2.0 ** -14
+    mid_half = 2.0 ** -17 if ew.fmt == "bf16" else 0.0
     for t in range(x.shape[0]):
         for j in range(topk):
             e = int(ids[t, j])
             xd = x[t].double()
-            h1, s1 = w1[e] @ xd, (w1[e].abs() @ xd.abs()) * (xd.numel() * 2.0 ** -23 + 2.0 ** -28)
+            h1, s1 = w1[e] @ xd, (w1[e].abs() @ (xd.abs() + digits * xd.abs().max())) * (xd.numel() * 2.0 ** -23)
+            s1 = s1 + w1[e].abs().sum(1) * digits * xd.abs().max()
             if ew.act == "swiglu":
                 gate, up = h1[0::2], h1[1::2]
                 mid = gate * torch.sigmoid(gate) * up
@@ -52,7 +55,7 @@ def _exact(ew, x, rx, router, topk, sigmoid, bias, scale, shared, renorm=True):
                 mid = torch.relu(h1) ** 2
                 d = 2 * h1.abs() * s1 + s1 ** 2
             d = d + 2.0 ** -18 * mid.abs()
-            d = d + mid_half * (mid.abs() + d) + 2.0 ** -28 * mid.abs().max()
+            d = d + mid_half * (mid.abs() + d) + digits * (mid.abs() + d).max()
             y, a = w2[e] @ mid, w2[e].abs()
             dy = a @ d + (a @ mid.abs()) * (mid.numel() * 2.0 ** -23)
             out[t] += w[t, j] * y
@@ -197,8 +200,8 @@ def test_strided_rows_wide_layers_and_outputs_gpu(fmt):
     for lead, width in ((8, 272), (3, 263)):
         wide = lambda v: torch.zeros(v.shape[0], width, dtype=v.dtype, device="cuda")[:, lead:lead + 256].copy_(v)   # noqa: E731
         assert torch.equal(moe.layer_forward(wide(x), wide(router), ewg, 2, shared=wide(sh)), want)
-    ew, x, rx, router, bias, sh = _case(16, 4, 8192, "relu2", fmt, 128, h_out=128, std=0.02)
-    assert nv.lib().hb_moe_few_tokens(moe._KINDS[fmt], 8192, 128, 4, moe.FC1_CLUSTER) < 16
+    ew, x, rx, router, bias, sh = _case(16, 4, 4608, "relu2", fmt, 128, h_out=128, std=0.02)
+    assert 8 <= nv.lib().hb_moe_few_tokens(moe._KINDS[fmt], 4608) < 16
     got = moe.layer_forward(x.cuda(), router.cuda(), ew.to("cuda"), 2, shared=sh.cuda())
     _check(got, *_exact(ew, x, None, router, 2, False, bias, 1.0, sh))
 
