@@ -47,6 +47,7 @@ constexpr int MAX_STAGES = 10;
 constexpr int MAX_SMEM = 227 * 1024;
 constexpr int A_BYTES = 128 * 128;       // 128 weight rows x 128 bytes of K
 constexpr int CANDIDATES = 128;          // of a token's top-k
+constexpr int CAND_BYTES = (2 * CANDIDATES + MAX_TOPK) * 4;
 
 template <int KIND>
 struct Traits {
@@ -449,13 +450,13 @@ __device__ __forceinline__ void warp_topk(const FewParams& p, const float* logit
 // ---------------------------------------------------------------- the experts' products
 __host__ __device__ constexpr int align_to(int v, int a) { return (v + a - 1) / a * a; }
 constexpr int BAR_BYTES = (3 * MAX_STAGES + 8) * 8;
-// Shared memory, from a 1024-byte boundary on: fc1: B tiles of x | stages (the candidates of the top-k before them) | scales of x | plan |
-// barriers; fc2: stages | sums [2][tokens][128] | plan | barriers
+// Shared memory, from a 1024-byte boundary on: fc1: B tiles of x | stages | scales of x | candidates of the top-k | plan | barriers;
+// fc2: stages | sums [2][tokens][128] | plan | barriers
 __host__ __device__ inline int k_tiles_of(int k, int tile) { return (k + tile - 1) / tile; }
 template <int KIND>
-__host__ __device__ inline int fc1_fixed_bytes(int n, int hidden) {
+__host__ __device__ inline int fc1_fixed_bytes(int tokens, int n, int hidden) {
   using T = Traits<KIND>;
-  return 1024 + k_tiles_of(hidden, T::TILE_K) * (n * 128 + T::SF_BYTES) + align_to(sizeof(Plan), 16) + BAR_BYTES;
+  return 1024 + k_tiles_of(hidden, T::TILE_K) * (n * 128 + T::SF_BYTES) + tokens * CAND_BYTES + align_to(sizeof(Plan), 16) + BAR_BYTES;
 }
 template <int KIND>
 __host__ __device__ inline int fc2_fixed_bytes(int tokens) {
@@ -480,7 +481,7 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
   uint8_t* after = ring + S * STAGE;
   float* sums = reinterpret_cast<float*>(after);                                // fc2: [2][tokens][128]
   uint8_t* xsf = after;                                                         // fc1
-  uint8_t* plan_at = after + (SECOND ? 2 * p.tokens * 512 : xsf_bytes);
+  uint8_t* plan_at = after + (SECOND ? 2 * p.tokens * 512 : xsf_bytes + p.tokens * CAND_BYTES);
   Plan& plan = *reinterpret_cast<Plan*>(plan_at);
   uint64_t* full = reinterpret_cast<uint64_t*>(plan_at + align_to(sizeof(Plan), 16));
   uint64_t* empty = full + MAX_STAGES;
@@ -539,7 +540,7 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
     }
     __syncwarp();
     if (warp < p.tokens) {
-      uint32_t* cand = reinterpret_cast<uint32_t*>(ring) + warp * (2 * CANDIDATES + 32);
+      uint32_t* cand = reinterpret_cast<uint32_t*>(xsf + xsf_bytes + warp * CAND_BYTES);
       const float* logit = p.logits + warp * p.experts;
       int id;
       float w;
@@ -557,16 +558,17 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
       }
     }
   }
-  fence_proxy_async_smem();                   // candidates lay where weights are copied to
   make_plan(plan, p.tokens, p.topk);
 
   // Units: fc1: (entry, 128 weight rows), round the CTAs; fc2: the entries of this CTA of the cluster, on its 128 output rows.
   const int rows_per_expert = SECOND ? p.h_out : p.swiglu ? 2 * p.inter : p.inter;
   const int tiles = SECOND ? 1 : (rows_per_expert + 127) / 128;
-  const int units = plan.entries * tiles;
-  const int u0 = SECOND ? static_cast<int>(cluster_rank) : static_cast<int>(blockIdx.x);
-  const int stride = SECOND ? static_cast<int>(cluster_n) : static_cast<int>(gridDim.x);
-  const int out_block = SECOND ? static_cast<int>(blockIdx.x / cluster_n) : 0;
+  // (shuffled, so that the compiler knows that the warps' loops are uniform: the operands of tcgen05 and TMA instructions then live
+  // in uniform registers. Bounds straight from shared memory cost 0.45 us per K tile, more than its bytes take.)
+  const int units = __shfl_sync(0xffffffffu, plan.entries, 0) * tiles;
+  const int u0 = SECOND ? __shfl_sync(0xffffffffu, static_cast<int>(cluster_rank), 0) : static_cast<int>(blockIdx.x);
+  const int stride = SECOND ? __shfl_sync(0xffffffffu, static_cast<int>(cluster_n), 0) : static_cast<int>(gridDim.x);
+  const int out_block = SECOND ? static_cast<int>(blockIdx.x) / stride : 0;
 
   if constexpr (SECOND && KIND == kGemmNvfp4) {          // the largest exponent of every row this CTA reads
     const int n_exp = ((p.swiglu ? 2 * p.inter : p.inter) + 31) / 32;
@@ -581,18 +583,18 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
     __syncthreads();
   }
 
-  const uint32_t ring_addr = __shfl_sync(0xffffffffu, smem_u32(ring), 0);
+  const uint32_t ring_addr = __shfl_sync(0xffffffffu, smem_u32(ring), 0), xsf_addr = __shfl_sync(0xffffffffu, smem_u32(xsf), 0);
   if (warp == 0) {
     // ---- weights: the whole warp walks the loop (waits included), one elected lane issues
-    int i = 0, issued = 0;
+    int i = 0, s = 0;
+    uint32_t phase = 1;                       // (the first round finds every stage free)
     bool ok = true;
     for (int u = u0; u < units && ok; u += stride) {
       const int entry = u / tiles;
       const int row0 = __shfl_sync(0xffffffffu, static_cast<int>(plan.expert[entry]) * rows_per_expert +
                                                     (SECOND ? out_block : u - entry * tiles) * 128, 0);
       for (int kt = 0; kt < k_tiles; ++kt, ++i) {
-        const int s = i % S;
-        if (i >= S) ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ((i / S) & 1) ^ 1, abort, p.status, kTimeoutEmpty));
+        ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], phase, abort, p.status, kTimeoutEmpty));
         if (!ok) break;
         if (elect_one()) {
           const uint32_t st = ring_addr + s * STAGE, bar = smem_u32(&full[s]);
@@ -603,18 +605,22 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
                       T::SF_BYTES, bar);
         }
         __syncwarp();
-        issued = i + 1;
+        if (++s == S) {
+          s = 0;
+          phase ^= 1;
+        }
       }
     }
     if (!ok && lane == 0) {                   // bounded wait for the copies still in flight: none may land after the CTA has gone
       volatile int ignore = 0;
-      for (int j = max(issued - S, 0); j < issued; ++j) mbar_wait(&full[j % S], (j / S) & 1, &ignore, nullptr, kTimeoutDrain);
+      for (int j = max(i - S, 0); j < i; ++j) mbar_wait(&full[j % S], (j / S) & 1, &ignore, nullptr, kTimeoutDrain);
     }
     __syncwarp();
   } else if (warp == 1) {
     // ---- products
-    int i = 0, it = 0;
-    bool ok = true;
+    int s = 0, it = 0;
+    uint32_t phase = 0;
+    bool ok = true, ready = false;
     if constexpr (!SECOND) ok = __all_sync(0xffffffffu, mbar_wait(x_full, 0, abort, p.status, kTimeoutFull));
     for (int u = u0; u < units && ok; u += stride, ++it) {
       const int n = __shfl_sync(0xffffffffu, SECOND ? (plan.count[u] * P + 15) / 16 * 16 : p.n, 0);
@@ -622,19 +628,27 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
       if (it >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&acc_free[it & 1], ((it >> 1) - 1) & 1, abort, p.status, kTimeoutAccum));
       if (!ok) break;
       tc_fence_after();
-      for (int kt = 0; kt < k_tiles; ++kt, ++i) {
-        const int s = i % S;
-        ok = __all_sync(0xffffffffu, mbar_wait(&full[s], (i / S) & 1, abort, p.status, kTimeoutFull));
-        if (SECOND && ok) ok = __all_sync(0xffffffffu, mbar_wait(&b_full[s], (i / S) & 1, abort, p.status, kTimeoutFull));
+      for (int kt = 0; kt < k_tiles; ++kt) {
+        if (!ready) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&full[s], phase, abort, p.status, kTimeoutFull));
+          if (SECOND && ok) ok = __all_sync(0xffffffffu, mbar_wait(&b_full[s], phase, abort, p.status, kTimeoutFull));
+        }
         if (!ok) break;
         tc_fence_after();
-        const uint32_t st = ring_addr + s * STAGE;
+        const int s_at = s;
+        if (++s == S) {
+          s = 0;
+          phase ^= 1;
+        }
+        // of the next tile, answered while this one is issued: a wait that finds its barrier complete takes 0.1 us all the same
+        const bool peek = mbar_test_wait(&full[s], phase) && (!SECOND || mbar_test_wait(&b_full[s], phase));
+        const uint32_t st = ring_addr + s_at * STAGE;
         const uint32_t b_at = SECOND ? st + A_BYTES + T::SF_BYTES * 2 : ring_addr - x_bytes + kt * p.n * 128;
         const uint64_t adesc = make_desc_sw128(st), bdesc = make_desc_sw128(b_at);
         const int mmas = min(4, (K - kt * T::TILE_K + T::MMA_K - 1) / T::MMA_K);
         if (elect_one()) {
           if constexpr (T::kFp4) {
-            const uint32_t sfb = SECOND ? st + A_BYTES + T::SF_BYTES : smem_u32(xsf) + kt * T::SF_BYTES;
+            const uint32_t sfb = SECOND ? st + A_BYTES + T::SF_BYTES : xsf_addr + kt * T::SF_BYTES;
 #pragma unroll
             for (int at = 0; at < T::ATOMS; ++at) {
               tmem_cp_32x128b_x4(tmem + SFA_COL + at * 4, make_desc_sf(st + A_BYTES + at * 512));
@@ -654,10 +668,10 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
             else
               mma_f16(acc, adesc + kb * 2, bdesc + kb * 2, make_idesc_bf16(128, 0) | static_cast<uint32_t>(n >> 3) << 17, more);
           }
-          tc_commit(&empty[s]);
+          tc_commit(&empty[s_at]);
           if (kt == k_tiles - 1) tc_commit(&accum[it & 1]);
         }
-        __syncwarp();
+        ready = __all_sync(0xffffffffu, peek);
       }
     }
   } else if (warp >= 4 && warp < 12) {
@@ -709,16 +723,23 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
   } else if (SECOND) {
     // ---- rows of mid: converter j writes the B tile of every CONVERTERS-th K tile
     const int j = warp < 4 ? warp - 2 : warp - 10;
-    int i = 0;
+    int next = j, s = 0;                      // tiles until this warp's next one; the stage of the tile at hand
+    uint32_t phase = 1;
     bool ok = true;
     for (int u = u0; u < units && ok; u += stride) {
       const int n = plan.count[u];
-      for (int kt = 0; kt < k_tiles; ++kt, ++i) {
-        if (i % CONVERTERS != j) continue;
-        const int s = i % S;
-        if (i >= S) ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ((i / S) & 1) ^ 1, abort, p.status, kTimeoutEmpty));
+      for (int kt = 0; kt < k_tiles; ++kt) {
+        const int mine = s;
+        const uint32_t turn = phase;
+        if (++s == S) {
+          s = 0;
+          phase ^= 1;
+        }
+        if (next-- != 0) continue;
+        next = CONVERTERS - 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(&empty[mine], turn, abort, p.status, kTimeoutEmpty));
         if (!ok) break;
-        uint8_t* sfb = ring + s * STAGE + A_BYTES + T::SF_BYTES;
+        uint8_t* sfb = ring + mine * STAGE + A_BYTES + T::SF_BYTES;
         uint8_t* b = sfb + T::SF_BYTES;
         if constexpr (T::kFp4) {
           const int k = kt * T::TILE_K + lane * 8;
@@ -760,7 +781,7 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&b_full[s]);
+        if (lane == 0) mbar_arrive(&b_full[mine]);
       }
     }
   }
@@ -819,8 +840,8 @@ int resident(int size) {
 }
 
 template <int KIND>
-int fc1_stages(int n, int hidden) {
-  return std::min(MAX_STAGES, (MAX_SMEM - fc1_fixed_bytes<KIND>(n, hidden)) / Traits<KIND>::STAGE1);
+int fc1_stages(int tokens, int n, int hidden) {
+  return std::min(MAX_STAGES, (MAX_SMEM - fc1_fixed_bytes<KIND>(tokens, n, hidden)) / Traits<KIND>::STAGE1);
 }
 int columns(int tokens, int per) { return (tokens * per + 15) / 16 * 16; }
 
@@ -828,7 +849,7 @@ int columns(int tokens, int per) { return (tokens * per + 15) / 16 * 16; }
 template <int KIND>
 int most_tokens(int hidden) {
   for (int t = MAX_TOKENS; t > 0; --t)
-    if (fc1_stages<KIND>(columns(t, Traits<KIND>::XP), hidden) >= 3) return t;
+    if (fc1_stages<KIND>(t, columns(t, Traits<KIND>::XP), hidden) >= 3) return t;
   return 0;
 }
 
@@ -885,7 +906,7 @@ cudaError_t launch_few(FewParams& p, const void* w1, const void* w2, uint8_t* ws
   if (!map(w1, n1, p.hidden, &t1) || !map(w2, p.h_out, p.inter, &t2)) return cudaErrorInvalidValue;
   cudaError_t e = launch_dep(moe_few_route_kernel<KIND>, dim3((p.experts + 15) / 16 + p.tokens), dim3(ROUTE_WARPS * 32), 0, st, p);
   if (e != cudaSuccess) return e;
-  p.stages = fc1_stages<KIND>(p.n, p.hidden);
+  p.stages = fc1_stages<KIND>(p.tokens, p.n, p.hidden);
   e = launch_dep(k1, dim3(kNumSms), dim3(THREADS), MAX_SMEM, st, t1, p);
   if (e != cudaSuccess) return e;
   p.stages = std::min(MAX_STAGES, (MAX_SMEM - fc2_fixed_bytes<KIND>(p.tokens)) / T::STAGE2);

@@ -50,6 +50,12 @@ def set_pdl(on) -> None:
 
 
 
+def init_pdl() -> None:
+    """The configured launch level, before the first kernel of a process that asks for it."""
+    if not _PDL_INIT:
+        set_pdl(cfgmod.current().pdl)
+
+
 def _plan(m: int, n: int, k_tiles: int, max_ws_bytes: int) -> tuple[bool, int, int]:
     """(swap, bn, splits) for an [m tokens] x [n features] problem. Negative splits: the launch may lower their number to
     fit the chip, but by the same amount at every tile width."""

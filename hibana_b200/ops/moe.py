@@ -507,6 +507,7 @@ def layer_forward(x: torch.Tensor, router: torch.Tensor, ew: ExpertWeights, topk
 
 def _few_launch(kind, x, rx, router, ew, topk, ra, sel_bias, shared, out) -> None:
     t, lib = x.shape[0], nv.lib()
+    gemm.init_pdl()
     ws = torch.empty(lib.hb_moe_few_ws(kind, t, ew.experts, topk, ew.hidden, ew.inter), dtype=torch.uint8, device=x.device)
     if kind == 0:
         w1, w2 = (ew.fc1.data_ptr(), None, None, 0), (ew.fc2.data_ptr(), None, None, 0)
