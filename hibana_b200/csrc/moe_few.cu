@@ -26,6 +26,7 @@
 // rows) over all CTAs with all tokens' columns resident; in fc2 the CTAs of a cluster share an output block of 128 rows, each with its
 // part of the experts, and add up through distributed shared memory in order.
 #include <algorithm>
+#include <cstddef>
 
 #include "gemm.cuh"
 #include "hb_api.h"
@@ -82,26 +83,33 @@ struct FewParams {
   float* logits;                         // [tokens][experts]
   float* x_factor;                       // [tokens] NVFP4: what the blocks' scales of a row are relative to
   uint8_t* x_img;                        // [K tiles][n][128] swizzled B tiles, then [K tiles][SF_BYTES] scales
-  int* ids;                              // [pairs]
-  float* weights;
+  struct EntryRecord* entries;           // [pairs] the plan, for fc2
   float* mid;                            // [pairs][inter]
   uint8_t* mid_exp;                      // [pairs][exp_ld] biased exponent of the largest number of 32 rows of fc1 (NVFP4)
   int exp_ld, n, stages;
   int* status;
 };
 
-// The routing as every CTA holds it: entries (an expert and up to eight of its tokens) in ascending order of experts.
+// The routing as every CTA holds it: entries, an expert and up to eight of its tokens, in the order in which the tokens' lists first
+// name them.
 struct Plan {
   int entries;
   int ids[MAX_PAIRS];
   float weights[MAX_PAIRS];
-  uint32_t chosen[MAX_TOKENS][MAX_EXPERTS / 32];     // bit e: the token chose expert e
-  uint32_t any[MAX_EXPERTS / 32], two[MAX_EXPERTS / 32];   // some token, more than eight tokens did
-  int before[MAX_EXPERTS / 32];                       // entries of the experts below 32 w
-  unsigned short expert[MAX_PAIRS], count[MAX_PAIRS];     // of entries
-  unsigned short pair[MAX_PAIRS * COLS];              // [entry][column]: token * topk + j
-  int row_exp[MAX_PAIRS];                             // fc2, NVFP4: exponent of the row's largest number
+  uint32_t chosen[MAX_TOKENS][MAX_EXPERTS / 32];      // bit e: the token chose expert e
+  int starts[THREADS / 32];
+  unsigned short entry_of[MAX_EXPERTS * 2];             // entry of an expert's tokens 0 .. 7, 8 .. 15
+  unsigned short expert[MAX_PAIRS], count[MAX_PAIRS];   // of entries
+  alignas(16) unsigned short pair[MAX_PAIRS * COLS];    // [entry][column]: token * topk + j
+  int row_exp[MAX_PAIRS];                               // fc2, NVFP4: exponent of the row's largest number
 };
+static_assert(alignof(Plan) == 16, "entries are stored as 16-byte pieces");
+struct alignas(16) EntryRecord {
+  int expert, count, entries, unused;
+  unsigned short pair[COLS];
+  float weight[COLS];
+};
+static_assert(sizeof(EntryRecord) == 64 && offsetof(EntryRecord, pair) == 16 && offsetof(EntryRecord, weight) == 32, "read in 16-byte pieces");
 
 // ---------------------------------------------------------------- rows of activations as operand B
 // Byte of K element `k` (of the K tile) in row n of a B tile: 128-byte rows, 16-byte chunks permuted by the row (SWIZZLE_128B).
@@ -175,7 +183,7 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a
 // ---------------------------------------------------------------- route
 // CTAs up to experts / 16: the logits of sixteen experts, K split over the warps. A lane holds eight consecutive K of two router rows
 // and of a token, so K is permuted alike on both sides of the products. The others: one row of x each.
-constexpr int ROUTE_WARPS = 8;
+constexpr int ROUTE_WARPS = 16;
 template <int KIND>
 __global__ void __launch_bounds__(ROUTE_WARPS * 32) moe_few_route_kernel(const __grid_constant__ FewParams p) {
   using T = Traits<KIND>;
@@ -226,7 +234,7 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) moe_few_route_kernel(const _
     }
     __syncthreads();
     const int tok = tid >> 4, e = e0 + (tid & 15);
-    if (tok < p.tokens && e < p.experts) {
+    if (tid < 256 && tok < p.tokens && e < p.experts) {
       float s = 0.f;
 #pragma unroll
       for (int w = 0; w < ROUTE_WARPS; ++w) s += part[w][tid];
@@ -278,56 +286,37 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) moe_few_route_kernel(const _
 }
 
 // ---------------------------------------------------------------- plan
-// Entries of the routing in plan.ids, by a whole CTA. Everything is bit masks over the experts, so nothing depends on timing.
+// Entries of the routing in plan.ids and plan.chosen, by a whole CTA. Bit masks and ballots: nothing depends on timing.
 __device__ __forceinline__ void make_plan(Plan& plan, int tokens, int topk) {
-  const int tid = threadIdx.x, lane = tid & 31, pairs = tokens * topk;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, pairs = tokens * topk;
   static_assert(THREADS == MAX_TOKENS * MAX_EXPERTS / 32 && THREADS >= MAX_PAIRS, "one mask word, one pair a thread");
-  plan.chosen[tid >> 5][lane] = 0;
   __syncthreads();
   const int my_token = tid / topk, e = tid < pairs ? plan.ids[tid] : 0;
-  if (tid < pairs) atomicOr(&plan.chosen[my_token][e >> 5], 1u << (e & 31));
-  __syncthreads();
-  if (tid < 32) {
-    uint32_t c[5] = {0, 0, 0, 0, 0};           // how many tokens chose each of this word's experts, bit by bit
-    for (int t = 0; t < tokens; ++t) {
-      uint32_t carry = plan.chosen[t][lane];
-#pragma unroll
-      for (int i = 0; i < 5; ++i) {
-        const uint32_t both = c[i] & carry;
-        c[i] ^= carry;
-        carry = both;
-      }
-    }
-    const uint32_t any = c[0] | c[1] | c[2] | c[3] | c[4], two = c[4] | (c[3] & (c[0] | c[1] | c[2]));
-    const int mine = __popc(any) + __popc(two);
-    int inc = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += up;
-    }
-    plan.any[lane] = any;
-    plan.two[lane] = two;
-    plan.before[lane] = inc - mine;
-    if (lane == 31) plan.entries = inc;
-  }
-  __syncthreads();
+  int slot = 1, all = 0;                       // tokens before this one that chose the expert, and all that did
   if (tid < pairs) {
-    const int w = e >> 5, b = e & 31;
-    const uint32_t below = (1u << b) - 1u;
-    int slot = 0, all = 0;                     // tokens before this one that chose the expert, and all that did
+    slot = 0;
     for (int t = 0; t < tokens; ++t) {
-      const int in = (plan.chosen[t][w] >> b) & 1;
+      const int in = (plan.chosen[t][e >> 5] >> (e & 31)) & 1;
       all += in;
       slot += t < my_token ? in : 0;
     }
-    const int entry = plan.before[w] + __popc(plan.any[w] & below) + __popc(plan.two[w] & below) + slot / COLS;
-    plan.pair[entry * COLS + slot % COLS] = static_cast<unsigned short>(tid);
-    if (slot % COLS == 0) {
-      plan.expert[entry] = static_cast<unsigned short>(e);
-      plan.count[entry] = static_cast<unsigned short>(min(COLS, all - slot));
-    }
   }
+  const bool start = slot % COLS == 0;
+  const uint32_t starts = __ballot_sync(0xffffffffu, start);
+  if (lane == 0) plan.starts[warp] = __popc(starts);
+  __syncthreads();
+  int before = lane < THREADS / 32 ? plan.starts[lane] : 0;
+  const int total = __reduce_add_sync(0xffffffffu, before);
+  const int entry = __reduce_add_sync(0xffffffffu, lane < warp ? before : 0) + __popc(starts & ((1u << lane) - 1u));
+  if (tid == 0) plan.entries = total;
+  if (start) {
+    plan.expert[entry] = static_cast<unsigned short>(e);
+    plan.count[entry] = static_cast<unsigned short>(min(COLS, all - slot));
+    plan.pair[entry * COLS] = static_cast<unsigned short>(tid);
+    plan.entry_of[e * 2 + slot / COLS] = static_cast<unsigned short>(entry);
+  }
+  __syncthreads();
+  if (tid < pairs && !start) plan.pair[plan.entry_of[e * 2 + slot / COLS] * COLS + slot % COLS] = static_cast<unsigned short>(tid);
   __syncthreads();
 }
 
@@ -336,44 +325,28 @@ __device__ __forceinline__ uint32_t order_key(float v) {          // orders floa
   return max((b & 0x80000000u) ? ~b : (b | 0x80000000u), 1u);
 }
 
-// Top-k of one token by one warp, PER experts a lane. Lane j < topk returns id and weight; scores, order and weights are those of
-// moe_route_kernel (moe.cu). No lane whose best key is below the topk-th largest of the 32 lanes' best keys can hold a chosen
-// expert, so a few candidates are left, which rank themselves; where they are more than CANDIDATES, one by one.
+// Top-k of one token by one warp, PER experts a lane. Lane j < topk returns id and weight, in descending order of score (+ bias), ties
+// by the lower id, as `route` orders them; softmax scores are ordered by their logits, and only the chosen ones' (renorm) are
+// computed. No lane whose best key is below the topk-th largest of the 32 lanes' best keys can hold a chosen expert, so a few
+// candidates are left, which rank themselves; where they are more than CANDIDATES (many equal scores), they are taken one by one.
 template <int PER>
 __device__ __forceinline__ void warp_topk(const FewParams& p, const float* logit, uint32_t* cand_key, uint32_t* cand_id, int& id,
                                           float& weight) {
   const int lane = threadIdx.x & 31, E = p.experts, K = p.topk;
-  const uint32_t below = (1u << lane) - 1u;
   float s[PER];
   uint32_t key[PER], best = 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) s[i] = i * 32 + lane < E ? ld_step(logit + i * 32 + lane) : -INFINITY;
-  if (p.sigmoid) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int e = i * 32 + lane;
-      const float b = p.sel_bias != nullptr && e < E ? __ldg(p.sel_bias + e) : 0.f;
-      s[i] = 1.f / (1.f + __expf(-s[i]));
-      key[i] = e < E ? order_key(s[i] + b) : 0u;
-      best = max(best, key[i]);
+  for (int i = 0; i < PER; ++i) {
+    const int e = i * 32 + lane;
+    float v = s[i];
+    if (p.sigmoid) {
+      s[i] = __fdividef(1.f, 1.f + __expf(-v));
+      v = s[i] + (p.sel_bias != nullptr && e < E ? __ldg(p.sel_bias + e) : 0.f);
     }
-  } else {
-    float mx = -INFINITY, sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) mx = fmaxf(mx, s[i]);
-    mx = warp_max(mx);
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      s[i] = i * 32 + lane < E ? __expf(s[i] - mx) : 0.f;
-      sum += s[i];
-    }
-    const float inv = 1.f / warp_sum(sum);
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      s[i] *= inv;
-      key[i] = i * 32 + lane < E ? order_key(s[i]) : 0u;
-      best = max(best, key[i]);
-    }
+    key[i] = e < E ? order_key(v) : 0u;
+    best = max(best, key[i]);
   }
   int rank = 0;
 #pragma unroll
@@ -382,69 +355,78 @@ __device__ __forceinline__ void warp_topk(const FewParams& p, const float* logit
     rank += other > best || (other == best && i < lane);
   }
   const uint32_t thr = max(__shfl_sync(0xffffffffu, best, __ffs(__ballot_sync(0xffffffffu, rank == K - 1)) - 1), 1u);
-  int n = 0, ties = 0;               // of equal keys at the threshold the first K will do
+  int mine = 0;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {    // ascending experts
-    const uint32_t eq = __ballot_sync(0xffffffffu, key[i] == thr);
-    const bool take = key[i] > thr || (key[i] == thr && ties + __popc(eq & below) < K);
-    const uint32_t taken = __ballot_sync(0xffffffffu, take);
-    const int at = n + __popc(taken & below);
-    if (take && at < CANDIDATES) {
-      cand_key[at] = key[i];
-      cand_id[at] = i * 32 + lane;
-    }
-    n += __popc(taken);
-    ties += __popc(eq);
+  for (int i = 0; i < PER; ++i) mine += key[i] >= thr;
+  int at = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, at, o);
+    if (lane >= o) at += up;
   }
+  const int n = __shfl_sync(0xffffffffu, at, 31);
+  at -= mine;
   id = 0;
   if (n <= CANDIDATES) {
-    const int pad = (n + 3) & ~3;
-    if (lane < pad - n) cand_key[n + lane] = 0;      // (pad <= CANDIDATES)
-    __syncwarp();
-    for (int c0 = 0; c0 < n; c0 += 32) {              // a candidate's place (the list ascends: of equal keys the earlier goes first)
-      const int c = c0 + lane;
-      const uint32_t mine = c < n ? cand_key[c] : 0u;
-      int place = 0;
-#pragma unroll 2
-      for (int i = 0; i < pad; i += 4) {
-        const uint4 k = *reinterpret_cast<const uint4*>(cand_key + i);
-        place += (k.x > mine || (k.x == mine && i < c)) + (k.y > mine || (k.y == mine && i + 1 < c)) +
-                 (k.z > mine || (k.z == mine && i + 2 < c)) + (k.w > mine || (k.w == mine && i + 3 < c));
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (key[i] >= thr) {
+        cand_key[at] = key[i];
+        cand_id[at++] = i * 32 + lane;
       }
-      const uint32_t e = c < n ? cand_id[c] : 0u;
-      // everybody has read this round's list entries it needs from others only above: ids move through the upper half
-      if (c < n && place < K) cand_id[CANDIDATES + place] = e;
+    __syncwarp();
+    for (int c = lane; c < n; c += 32) {
+      const uint32_t k = cand_key[c], e = cand_id[c];
+      int place = 0;
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) {
+        const uint32_t ok = cand_key[i], oe = cand_id[i];
+        place += ok > k || (ok == k && oe < e);
+      }
+      if (place < K) cand_id[CANDIDATES + place] = e;
     }
     __syncwarp();
     if (lane < K) id = static_cast<int>(cand_id[CANDIDATES + lane]);
   } else {
     for (int j = 0; j < K; ++j) {
-      uint32_t mine = 0;
-      int at = lane;
+      uint32_t top_mine = 0;
+      int e = lane;
 #pragma unroll
       for (int i = PER - 1; i >= 0; --i)
-        if (key[i] >= mine && key[i] != 0) {
-          mine = key[i];
-          at = i * 32 + lane;
+        if (key[i] >= top_mine && key[i] != 0) {
+          top_mine = key[i];
+          e = i * 32 + lane;
         }
-      const uint32_t top = __reduce_max_sync(0xffffffffu, mine);
-      const int win = static_cast<int>(__reduce_min_sync(0xffffffffu, mine == top ? static_cast<uint32_t>(at) : 0x7FFFFFFFu));
+      const uint32_t top = __reduce_max_sync(0xffffffffu, top_mine);
+      const int win = static_cast<int>(__reduce_min_sync(0xffffffffu, top_mine == top ? static_cast<uint32_t>(e) : 0x7FFFFFFFu));
       if (lane == j) id = win;
 #pragma unroll
       for (int i = 0; i < PER; ++i)
         if (i * 32 + lane == win) key[i] = 0;
     }
   }
-  // the chosen ones' scores: lane id % 32 has the one of expert `id` in s[id / 32]
-  weight = 0.f;
+  // the chosen ones' scores (softmax: logits so far): lane id % 32 has the one of expert `id` in s[id / 32]
+  weight = -INFINITY;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const float v = __shfl_sync(0xffffffffu, s[i], id & 31);
     if ((id >> 5) == i) weight = v;
   }
-  float sum = 0.f;
-  for (int j = 0; j < K; ++j) sum += __shfl_sync(0xffffffffu, weight, j);
-  weight = (p.renorm ? weight / fmaxf(sum, 1e-20f) : weight) * p.scale;
+  if (lane >= K) weight = -INFINITY;
+  if (!p.sigmoid) {
+    const float mx = __shfl_sync(0xffffffffu, weight, 0);
+    weight = __expf(weight - mx);
+    if (!p.renorm) {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) sum += __expf(s[i] - mx);
+      weight /= warp_sum(sum);
+    }
+  } else if (lane >= K) {
+    weight = 0.f;
+  }
+  if (p.renorm) weight = weight / fmaxf(warp_sum(weight), 1e-20f);
+  weight *= p.scale;
 }
 
 // ---------------------------------------------------------------- the experts' products
@@ -516,8 +498,11 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
     tmem_alloc(tmem_slot, TMEM_COLS);
     tmem_relinquish();
   }
-  if constexpr (SECOND)
+  if constexpr (SECOND) {
     for (int i = tid; i < 2 * p.tokens * 128; i += THREADS) sums[i] = 0.f;
+  } else {
+    (&plan.chosen[0][0])[tid] = 0;
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -527,10 +512,21 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
 
   const int pairs = p.tokens * p.topk;
   if constexpr (SECOND) {
-    if (tid < pairs) {
-      plan.ids[tid] = ld_step(p.ids + tid);
-      plan.weights[tid] = ld_step(p.weights + tid);
+    if (tid < pairs) {                        // (records past the last entry hold anything: nobody asks for them)
+      const EntryRecord* rec = p.entries + tid;
+      const uint4 head = ld_step(reinterpret_cast<const uint4*>(rec)), cols = ld_step(reinterpret_cast<const uint4*>(rec->pair));
+      const uint4 w0 = ld_step(reinterpret_cast<const uint4*>(rec->weight)), w1 = ld_step(reinterpret_cast<const uint4*>(rec->weight + 4));
+      const int entries = ld_step(&p.entries->entries);
+      if (tid == 0) plan.entries = entries;
+      plan.expert[tid] = static_cast<unsigned short>(head.x);
+      plan.count[tid] = static_cast<unsigned short>(head.y);
+      *reinterpret_cast<uint4*>(plan.pair + tid * COLS) = cols;
+      const uint32_t c[4] = {cols.x, cols.y, cols.z, cols.w}, w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+      for (int j = 0; j < COLS; ++j)
+        if (tid < entries && j < static_cast<int>(head.y)) plan.weights[(c[j >> 1] >> (16 * (j & 1))) & 0xFFFFu] = __uint_as_float(w[j]);
     }
+    __syncthreads();
   } else {
     if (warp == 15 && lane == 0) {            // (the last warp to get a token)
       mbar_expect_tx(x_full, x_bytes + xsf_bytes);
@@ -551,14 +547,25 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
         const int at = warp * p.topk + lane;
         plan.ids[at] = id;
         plan.weights[at] = w;
-        if (blockIdx.x == 0) {                // fc2 makes the same plan
-          p.ids[at] = id;
-          p.weights[at] = w;
-        }
+        atomicOr(&plan.chosen[warp][id >> 5], 1u << (id & 31));
       }
     }
+    make_plan(plan, p.tokens, p.topk);
+    if (blockIdx.x == 0 && tid < plan.entries) {
+      EntryRecord rec;
+      rec.expert = plan.expert[tid];
+      rec.count = plan.count[tid];
+      rec.entries = plan.entries;
+      rec.unused = 0;
+#pragma unroll
+      for (int j = 0; j < COLS; ++j) {
+        const bool in = j < rec.count;
+        rec.pair[j] = in ? plan.pair[tid * COLS + j] : 0;
+        rec.weight[j] = in ? plan.weights[rec.pair[j]] : 0.f;
+      }
+      p.entries[tid] = rec;
+    }
   }
-  make_plan(plan, p.tokens, p.topk);
 
   // Units: fc1: (entry, 128 weight rows), round the CTAs; fc2: the entries of this CTA of the cluster, on its 128 output rows.
   const int rows_per_expert = SECOND ? p.h_out : p.swiglu ? 2 * p.inter : p.inter;
@@ -845,16 +852,16 @@ int fc1_stages(int tokens, int n, int hidden) {
 }
 int columns(int tokens, int per) { return (tokens * per + 15) / 16 * 16; }
 
-// Most tokens of a call: at least three stages of weights beside the rows of x.
+// Most tokens of a call: at least two stages of weights beside the rows of x.
 template <int KIND>
 int most_tokens(int hidden) {
   for (int t = MAX_TOKENS; t > 0; --t)
-    if (fc1_stages<KIND>(t, columns(t, Traits<KIND>::XP), hidden) >= 3) return t;
+    if (fc1_stages<KIND>(t, columns(t, Traits<KIND>::XP), hidden) >= 2) return t;
   return 0;
 }
 
 struct WsLayout {
-  long long logits, factor, img, ids, weights, mid, exp, bytes;
+  long long logits, factor, img, entries, mid, exp, bytes;
   int exp_ld;
 };
 template <int KIND>
@@ -868,9 +875,8 @@ WsLayout ws_layout(int tokens, int experts, int topk, int hidden, int inter) {
   w.mid = up(static_cast<long long>(k_tiles_of(hidden, T::TILE_K)) * (columns(tokens, T::XP) * 128 + T::SF_BYTES));
   w.logits = w.mid + up(pairs * inter * 4);
   w.factor = w.logits + up(4ll * tokens * experts);
-  w.ids = w.factor + up(4ll * tokens);
-  w.weights = w.ids + up(4 * pairs);
-  w.exp = w.weights + up(4 * pairs);
+  w.entries = w.factor + up(4ll * tokens);
+  w.exp = w.entries + up(sizeof(EntryRecord) * pairs);
   w.bytes = w.exp + up(pairs * w.exp_ld);
   return w;
 }
@@ -891,8 +897,7 @@ cudaError_t launch_few(FewParams& p, const void* w1, const void* w2, uint8_t* ws
   p.mid = reinterpret_cast<float*>(ws + w.mid);
   p.logits = reinterpret_cast<float*>(ws + w.logits);
   p.x_factor = reinterpret_cast<float*>(ws + w.factor);
-  p.ids = reinterpret_cast<int*>(ws + w.ids);
-  p.weights = reinterpret_cast<float*>(ws + w.weights);
+  p.entries = reinterpret_cast<EntryRecord*>(ws + w.entries);
   p.mid_exp = ws + w.exp;
   p.exp_ld = w.exp_ld;
   p.n = columns(p.tokens, T::XP);
