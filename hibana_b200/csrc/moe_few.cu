@@ -45,9 +45,10 @@ constexpr int THREADS = WARPS * 32;
 constexpr int COLS = 8;                  // tokens of an entry of the plan
 constexpr int CONVERTERS = 6;            // warps 2, 3, 12 .. 15
 constexpr int MAX_STAGES = 10;
+constexpr int MAX_CLUSTER = 16;          // of fc2 (more than eight CTAs need a kernel attribute)
 constexpr int MAX_SMEM = 227 * 1024;
 constexpr int A_BYTES = 128 * 128;       // 128 weight rows x 128 bytes of K
-constexpr int CANDIDATES = 128;          // of a token's top-k
+constexpr int CANDIDATES = 64;           // of a token's top-k
 constexpr int CAND_BYTES = (2 * CANDIDATES + MAX_TOPK) * 4;
 
 template <int KIND>
@@ -325,46 +326,70 @@ __device__ __forceinline__ uint32_t order_key(float v) {          // orders floa
   return max((b & 0x80000000u) ? ~b : (b | 0x80000000u), 1u);
 }
 
-// Top-k of one token by one warp, PER experts a lane. Lane j < topk returns id and weight, in descending order of score (+ bias), ties
-// by the lower id, as `route` orders them; softmax scores are ordered by their logits, and only the chosen ones' (renorm) are
-// computed. No lane whose best key is below the topk-th largest of the 32 lanes' best keys can hold a chosen expert, so a few
-// candidates are left, which rank themselves; where they are more than CANDIDATES (many equal scores), they are taken one by one.
+// Top-k of one token by one warp, PER experts a lane. Lane j < topk returns id and weight, in descending order of score
+// (+ bias), ties by the lower id, as `route` orders them; softmax scores are ordered by their logits, and only the chosen ones'
+// (renorm) are computed. No lane whose best key is below the topk-th largest of the 32 lanes' best keys can hold a chosen
+// expert; that threshold is moved up until 32 candidates or fewer are left, which rank themselves. Where equal scores keep them
+// above CANDIDATES, they are found one by one.
 template <int PER>
 __device__ __forceinline__ void warp_topk(const FewParams& p, const float* logit, uint32_t* cand_key, uint32_t* cand_id, int& id,
                                           float& weight) {
   const int lane = threadIdx.x & 31, E = p.experts, K = p.topk;
   float s[PER];
   uint32_t key[PER], best = 0;
+  const bool biased = p.sigmoid && p.sel_bias != nullptr;
 #pragma unroll
   for (int i = 0; i < PER; ++i) s[i] = i * 32 + lane < E ? ld_step(logit + i * 32 + lane) : -INFINITY;
+  if (p.sigmoid) {
+    float b[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) b[i] = biased && i * 32 + lane < E ? ld_step(p.sel_bias + i * 32 + lane) : 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      s[i] = __fdividef(1.f, 1.f + __expf(-s[i]));
+      key[i] = order_key(s[i] + b[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) key[i] = order_key(s[i]);
+  }
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int e = i * 32 + lane;
-    float v = s[i];
-    if (p.sigmoid) {
-      s[i] = __fdividef(1.f, 1.f + __expf(-v));
-      v = s[i] + (p.sel_bias != nullptr && e < E ? __ldg(p.sel_bias + e) : 0.f);
-    }
-    key[i] = e < E ? order_key(v) : 0u;
+    key[i] = i * 32 + lane < E ? key[i] : 0u;
     best = max(best, key[i]);
   }
   int rank = 0;
-#pragma unroll
+#pragma unroll 8
   for (int i = 0; i < 32; ++i) {
     const uint32_t other = __shfl_sync(0xffffffffu, best, i);
     rank += other > best || (other == best && i < lane);
   }
-  const uint32_t thr = max(__shfl_sync(0xffffffffu, best, __ffs(__ballot_sync(0xffffffffu, rank == K - 1)) - 1), 1u);
-  int mine = 0;
+  uint32_t thr = max(__shfl_sync(0xffffffffu, best, __ffs(__ballot_sync(0xffffffffu, rank == K - 1)) - 1), 1u);
+  uint32_t high = __reduce_max_sync(0xffffffffu, best);
+  auto count = [&](uint32_t at_least) {
+    int c = 0;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) mine += key[i] >= thr;
+    for (int i = 0; i < PER; ++i) c += key[i] >= at_least;
+    return c;
+  };
+  int mine = count(thr), n = __reduce_add_sync(0xffffffffu, mine);
+  while (n > 32 && high - thr > 1) {        // at least K keys are >= thr all the time, fewer than K are >= high (or one value is left)
+    const uint32_t mid = thr + (high - thr) / 2;
+    const int c = count(mid), all = __reduce_add_sync(0xffffffffu, c);
+    if (all >= K) {
+      thr = mid;
+      mine = c;
+      n = all;
+    } else {
+      high = mid;
+    }
+  }
   int at = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int up = __shfl_up_sync(0xffffffffu, at, o);
     if (lane >= o) at += up;
   }
-  const int n = __shfl_sync(0xffffffffu, at, 31);
   at -= mine;
   id = 0;
   if (n <= CANDIDATES) {
@@ -412,7 +437,7 @@ __device__ __forceinline__ void warp_topk(const FewParams& p, const float* logit
     const float v = __shfl_sync(0xffffffffu, s[i], id & 31);
     if ((id >> 5) == i) weight = v;
   }
-  if (lane >= K) weight = -INFINITY;
+  if (lane >= K) weight = p.sigmoid ? 0.f : -INFINITY;
   if (!p.sigmoid) {
     const float mx = __shfl_sync(0xffffffffu, weight, 0);
     weight = __expf(weight - mx);
@@ -422,14 +447,22 @@ __device__ __forceinline__ void warp_topk(const FewParams& p, const float* logit
       for (int i = 0; i < PER; ++i) sum += __expf(s[i] - mx);
       weight /= warp_sum(sum);
     }
-  } else if (lane >= K) {
-    weight = 0.f;
   }
   if (p.renorm) weight = weight / fmaxf(warp_sum(weight), 1e-20f);
   weight *= p.scale;
 }
 
 // ---------------------------------------------------------------- the experts' products
+// Tile load of what is read once: first to leave L2, which holds instructions, activations and the router otherwise.
+__device__ __forceinline__ void tma_load_2d_once(uint32_t smem_dst, const CUtensorMap* m, uint32_t bar, int x, int y) {
+  asm volatile(
+      "{\n\t.reg .b64 pol;\n\t"
+      "createpolicy.fractional.L2::evict_first.b64 pol, 1.0;\n\t"
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4}], [%2], pol;\n\t}" ::"r"(
+          smem_dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
 __host__ __device__ constexpr int align_to(int v, int a) { return (v + a - 1) / a * a; }
 constexpr int BAR_BYTES = (3 * MAX_STAGES + 8) * 8;
 // Shared memory, from a 1024-byte boundary on: fc1: B tiles of x | stages | scales of x | candidates of the top-k | plan | barriers;
@@ -530,8 +563,7 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
   } else {
     if (warp == 15 && lane == 0) {            // (the last warp to get a token)
       mbar_expect_tx(x_full, x_bytes + xsf_bytes);
-      for (int kt = 0; kt < k_tiles; ++kt)
-        bulk_load(sm + kt * p.n * 128, p.x_img + static_cast<size_t>(kt) * p.n * 128, p.n * 128, x_full);
+      bulk_load(sm, p.x_img, x_bytes, x_full);      // (a copy takes this lane 0.3 us: tile by tile they held up the plan)
       if (xsf_bytes > 0) bulk_load(xsf, p.x_img + x_bytes, xsf_bytes, x_full);
     }
     __syncwarp();
@@ -606,7 +638,7 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
         if (elect_one()) {
           const uint32_t st = ring_addr + s * STAGE, bar = smem_u32(&full[s]);
           mbar_expect_tx(&full[s], A_BYTES + T::SF_BYTES);
-          tma_load_2d(st, &tw, bar, kt * (T::kFp4 ? 128 : 64), row0);
+          tma_load_2d_once(st, &tw, bar, kt * (T::kFp4 ? 128 : 64), row0);
           if constexpr (T::kFp4)
             bulk_load(st + A_BYTES, (SECOND ? p.sf2 : p.sf1) + (static_cast<size_t>(row0 >> 7) * (SECOND ? p.ka2 : p.ka1) + kt * T::ATOMS) * 512,
                       T::SF_BYTES, bar);
@@ -824,7 +856,7 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
 // Clusters of `size` CTAs of the second kernel that the chip holds at once (0: none).
 template <int KIND>
 int resident(int size) {
-  static int known[9] = {};              // + 1
+  static int known[MAX_CLUSTER + 1] = {};              // + 1
   if (known[size] == 0) {
     int n = 0;
     cudaLaunchConfig_t q = {};
@@ -889,6 +921,7 @@ cudaError_t launch_few(FewParams& p, const void* w1, const void* w2, uint8_t* ws
   static const cudaError_t ready = [&] {
     cudaError_t e = cudaFuncSetAttribute(k1, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SMEM);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k2, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SMEM);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k2, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     return e;
   }();
   if (ready != cudaSuccess) return ready;
@@ -919,7 +952,7 @@ cudaError_t launch_few(FewParams& p, const void* w1, const void* w2, uint8_t* ws
   const int blocks = (p.h_out + 127) / 128;
   int cluster = 1;
   double best = 1e30;
-  for (int c = 1; c <= 8; ++c) {
+  for (int c = 1; c <= MAX_CLUSTER; ++c) {
     const int room = resident<KIND>(c);
     if (room < 1) continue;
     const double cost = static_cast<double>((blocks + room - 1) / room) / c;

@@ -9,6 +9,7 @@ hibana/kernels/w3_moe.py:194 (reference), hibana/kernels/csrc/w3_gemm.cu:640-130
 """
 from __future__ import annotations
 
+import functools
 from dataclasses import dataclass
 from typing import Optional
 
@@ -439,11 +440,17 @@ def few_tokens_ref(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, ew
 
 
 def few_tokens_ok(ew: ExpertWeights, topk: int) -> bool:
-    """Whether the two-kernel form covers a layer: bf16, NVFP4 or MXFP4 experts, at most 1024 of them and 32 a token, with
+    """Whether the few-token form covers a layer: bf16, NVFP4 or MXFP4 experts, at most 1024 of them and 32 a token, with
     whole blocks (128 rows of FP4 weights and their scales) per expert and matrix."""
     rows, k = (8, 8) if ew.fmt == "bf16" else (128, 32)
     return (ew.fmt in _KINDS and ew.act in ("swiglu", "relu2") and ew.experts <= 1024 and topk <= 32 and ew.n1 % rows == 0
             and ew.fc2_rows % rows == 0 and ew.hidden % k == 0 and ew.inter % k == 0)
+
+
+@functools.lru_cache(maxsize=1024)
+def _few_sizes(kind: int, tokens: int, experts: int, topk: int, hidden: int, inter: int) -> tuple[int, int]:
+    """(most tokens of one call at this width, workspace bytes of a call of `tokens`)."""
+    return nv.lib().hb_moe_few_tokens(kind, hidden), nv.lib().hb_moe_few_ws(kind, tokens, experts, topk, hidden, inter)
 
 
 def _rows16(x: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -482,39 +489,44 @@ def layer_forward(x: torch.Tensor, router: torch.Tensor, ew: ExpertWeights, topk
         if other is not None and other.device != x.device:
             raise ValueError("layer_forward: operands on different devices")
     few = t <= FEW_TOKENS and few_tokens_ok(ew, topk)
-    route_args = {"sigmoid": sigmoid, "sel_bias": sel_bias, "renorm": renorm, "scale": scale}
     if not nv.use_native(x):
-        ids, w = route_ref(rx.float() @ router.float().t(), topk, **route_args)
+        ids, w = route_ref(rx.float() @ router.float().t(), topk, sigmoid=sigmoid, sel_bias=sel_bias, renorm=renorm, scale=scale)
         return few_tokens_ref(x, ids, w, ew, shared) if few else experts_forward(x, ids, w, ew, shared=shared)
     with nv.on_device(x):
         if t == 0:
             return torch.empty(0, ew.fc2_rows, dtype=torch.bfloat16, device=x.device)
         kind = _KINDS.get(ew.fmt, 0)
-        most = nv.lib().hb_moe_few_tokens(kind, ew.hidden) if few else 0       # (a wide layer's rows take several calls)
+        most = _few_sizes(kind, t, e, topk, ew.hidden, ew.inter)[0] if few else 0       # (a wide layer's rows take several calls)
         if most * 2 < t or router.shape[1] % 8:
-            ids, w = route(gemm.linear_bf16(rx, router, epilogue=gemm.EPI_STORE_F32), topk, **route_args)
+            ids, w = route(gemm.linear_bf16(rx, router, epilogue=gemm.EPI_STORE_F32), topk, sigmoid=sigmoid, sel_bias=sel_bias,
+                           renorm=renorm, scale=scale)
             return experts_forward(x, ids, w, ew, shared=shared)
         out = torch.empty(t, ew.fc2_rows, dtype=torch.bfloat16, device=x.device)
         x, router, shared = _rows16(x), _rows16(router), _rows16(shared)
         rx = x if route_x is None else _rows16(route_x)
         if sel_bias is not None:
             sel_bias = sel_bias.contiguous()
-        for lo in range(0, t, most):
-            _few_launch(kind, x[lo:lo + most], rx[lo:lo + most], router, ew, topk, route_args, sel_bias,
-                        None if shared is None else shared[lo:lo + most], out[lo:lo + most])
+        score = (int(sigmoid), int(renorm), scale)
+        if most >= t:
+            _few_launch(kind, x, rx, router, ew, topk, score, sel_bias, shared, out)
+        else:
+            for lo in range(0, t, most):
+                _few_launch(kind, x[lo:lo + most], rx[lo:lo + most], router, ew, topk, score, sel_bias,
+                            None if shared is None else shared[lo:lo + most], out[lo:lo + most])
     return out
 
 
-def _few_launch(kind, x, rx, router, ew, topk, ra, sel_bias, shared, out) -> None:
-    t, lib = x.shape[0], nv.lib()
+def _few_launch(kind, x, rx, router, ew, topk, score, sel_bias, shared, out) -> None:
+    t, dev = x.shape[0], x.device
     gemm.init_pdl()
-    ws = torch.empty(lib.hb_moe_few_ws(kind, t, ew.experts, topk, ew.hidden, ew.inter), dtype=torch.uint8, device=x.device)
+    e, h, i, fc1, fc2 = ew.experts, ew.hidden, ew.inter, ew.fc1, ew.fc2
+    ws = torch.empty(_few_sizes(kind, t, e, topk, h, i)[1], dtype=torch.uint8, device=dev)
     if kind == 0:
-        w1, w2 = (ew.fc1.data_ptr(), None, None, 0), (ew.fc2.data_ptr(), None, None, 0)
+        w1, w2 = (fc1.data_ptr(), None, None, 0), (fc2.data_ptr(), None, None, 0)
     else:
-        w1, w2 = ((w.q.data_ptr(), w.sf.data_ptr(), w.gscale.data_ptr() if kind == 1 else None, w.ka) for w in (ew.fc1, ew.fc2))
-    nv.check(lib.hb_moe_few(kind, x.data_ptr(), x.stride(0), rx.data_ptr(), rx.stride(0), router.data_ptr(), router.stride(0),
-                            router.shape[1], nv.ptr(sel_bias), t, ew.experts, topk, int(ra["sigmoid"]), int(ra["renorm"]),
-                            ra["scale"], ew.hidden, ew.inter, ew.fc2_rows, int(ew.act == "swiglu"), *w1, *w2, nv.ptr(shared),
-                            shared.stride(0) if shared is not None else 0, out.data_ptr(), out.stride(0), ws.data_ptr(),
-                            nv.device_state(x.device).status.data_ptr(), nv.stream()), "hb_moe_few", launches=3)
+        w1, w2 = ((w.q.data_ptr(), w.sf.data_ptr(), w.gscale.data_ptr() if kind == 1 else None, w.sf.shape[1]) for w in (fc1, fc2))
+    nv.check(nv.lib().hb_moe_few(kind, x.data_ptr(), x.stride(0), rx.data_ptr(), rx.stride(0), router.data_ptr(),
+                                 router.stride(0), router.shape[1], nv.ptr(sel_bias), t, e, topk, *score, h, i, out.shape[1],
+                                 int(ew.act == "swiglu"), *w1, *w2, nv.ptr(shared), 0 if shared is None else shared.stride(0),
+                                 out.data_ptr(), out.stride(0), ws.data_ptr(), nv.device_state(dev).status.data_ptr(),
+                                 nv.stream()), "hb_moe_few", launches=3)
