@@ -18,8 +18,8 @@
 // elements, 16 for NVFP4) is scaled by a power of two to 14-bit integers, X = sum_p d_p 8^p with digits d_p of -4 .. 4, which
 // e2m1 holds exactly. The digits of a row are five columns of the product (five rows of operand B, with the block's scale), and
 // the epilogue adds them up: 8^p D_p. What is lost is half a unit of X, 2^-14 to 2^-15 of the largest number of its block. An NVFP4
-// scale spans 2^-9 .. 2^8; blocks further below the largest of their row share the lowest one. With bf16 weights x is one column, and
-// mid two (two bf16 numbers, 16 bits).
+// scale spans 2^-9 .. 2^8; blocks further below the largest of their row share the lowest one. Rows of mid have one scale each, so that
+// half a unit is 2^-14 to 2^-15 of the row's largest number. With bf16 weights x is one column, and mid two (two bf16 numbers, 16 bits).
 //
 // Warp roles (fc1, fc2): one issues the weights' TMA copies into a ring of stages, one the MMAs, two groups of four read accumulators
 // back in turn; in fc2 six convert the rows of mid that a K tile needs, straight into the stage's B tile. fc1 walks (expert, 128
@@ -63,7 +63,7 @@ struct Traits {
   static constexpr int MP = kFp4 ? 5 : 2;
   static constexpr int B2_ROWS = (COLS * MP + 15) / 16 * 16;
   static constexpr int STAGE1 = A_BYTES + SF_BYTES;
-  static constexpr int STAGE2 = A_BYTES + B2_ROWS * 128 + 2 * SF_BYTES;
+  static constexpr int STAGE2 = A_BYTES + SF_BYTES + B2_ROWS * 128;
 };
 
 struct FewParams {
@@ -86,7 +86,7 @@ struct FewParams {
   uint8_t* x_img;                        // [K tiles][n][128] swizzled B tiles, then [K tiles][SF_BYTES] scales
   struct EntryRecord* entries;           // [pairs] the plan, for fc2
   float* mid;                            // [pairs][inter]
-  uint8_t* mid_exp;                      // [pairs][exp_ld] biased exponent of the largest number of 32 rows of fc1 (NVFP4)
+  uint8_t* mid_exp;                      // [pairs][exp_ld] biased exponent of the largest number of 32 rows of fc1 (FP4)
   int exp_ld, n, stages;
   int* status;
 };
@@ -102,7 +102,7 @@ struct Plan {
   unsigned short entry_of[MAX_EXPERTS * 2];             // entry of an expert's tokens 0 .. 7, 8 .. 15
   unsigned short expert[MAX_PAIRS], count[MAX_PAIRS];   // of entries
   alignas(16) unsigned short pair[MAX_PAIRS * COLS];    // [entry][column]: token * topk + j
-  int row_exp[MAX_PAIRS];                               // fc2, NVFP4: exponent of the row's largest number
+  int row_exp[MAX_PAIRS];                               // fc2, FP4: exponent of the row's largest number
 };
 static_assert(alignof(Plan) == 16, "entries are stored as 16-byte pieces");
 struct alignas(16) EntryRecord {
@@ -124,23 +124,8 @@ __device__ __forceinline__ uint32_t scale_byte(int e) {
   else return e == 128 ? 0x7Fu : e >= -6 ? static_cast<uint32_t>(e + 7) << 3 : 1u << (e + 9);
 }
 
-// Eight consecutive numbers of a block whose largest magnitude (bits) is `top` -> five words of eight e2m1 digits and the block's scale
-// byte. `row_e`: biased exponent of the row's largest number (NVFP4; 255 where the row holds an infinity or a NaN).
-template <int KIND>
-__device__ __forceinline__ uint32_t digits8(const float (&v)[8], uint32_t top, int row_e, uint32_t (&w)[5]) {
-  int e = static_cast<int>(top >> 23), scale;
-  if constexpr (KIND == kGemmMxfp4) {
-    const bool bad = e == 255;
-    e = max(e, 13);
-    scale = bad ? 128 : e - 140;           // X = v * 2^(140 - e), |X| <= 2^14
-  } else {
-    const bool bad = row_e == 255;
-    row_e = max(row_e, 13);
-    e = min(max(e, row_e - 17), row_e);
-    e = max(e, 13);
-    scale = bad ? 128 : e - row_e + 8;     // -9 .. 8
-  }
-  const float f = __int_as_float((267 - e) << 23);
+// Eight consecutive numbers times f (magnitudes of 2^14 at most) -> five words of eight e2m1 digits.
+__device__ __forceinline__ void digits8(const float (&v)[8], float f, uint32_t (&w)[5]) {
   // codes of the digits -4 .. 3 (4, which only the top digit takes, has code 6)
   constexpr uint32_t kCodes = 0x5420ACDEu;
 #pragma unroll
@@ -153,15 +138,32 @@ __device__ __forceinline__ uint32_t digits8(const float (&v)[8], uint32_t top, i
     const int top_digit = y >> 12;         // 0 .. 8
     w[4] |= (top_digit == 8 ? 6u : (kCodes >> (4 * top_digit)) & 15u) << (4 * j);
   }
-  return scale_byte<KIND>(scale);
 }
-// What the sum of digits times scales is to be multiplied by.
+// A block whose largest magnitude (bits) is `top`: the factor of its numbers, 2^(140 - e) with e the biased exponent of `top`, and the
+// block's scale byte. `row_e`: that exponent of the whole row (NVFP4), which x_factor undoes.
 template <int KIND>
-__device__ __forceinline__ float row_factor(int row_e) {
-  if constexpr (KIND != kGemmNvfp4) return 1.f;
-  const int e = max(min(row_e, 254), 13) - 148;      // -135 and up: a subnormal number below -126
+__device__ __forceinline__ float block_factor(uint32_t top, int row_e, uint32_t& scale) {
+  int e = static_cast<int>(top >> 23);
+  if constexpr (KIND == kGemmMxfp4) {
+    const bool bad = e == 255;
+    e = max(e, 13);
+    scale = scale_byte<KIND>(bad ? 128 : e - 140);
+  } else {
+    const bool bad = row_e == 255;
+    row_e = max(row_e, 13);
+    e = max(min(max(e, row_e - 17), row_e), 13);
+    scale = scale_byte<KIND>(bad ? 128 : e - row_e + 8);      // 2^-9 .. 2^8
+  }
+  return __int_as_float((267 - e) << 23);
+}
+__device__ __forceinline__ float pow2(int e) {              // -149 < e < 128
   return e >= -126 ? __int_as_float((e + 127) << 23) : __int_as_float(0x00400000 >> (-127 - e));
 }
+__device__ __forceinline__ float x_factor(int row_e) { return pow2(max(min(row_e, 254), 13) - 148); }
+// Rows of mid have one scale, that of their largest number (exponent e; 255: the row holds an infinity or a NaN, and all that is made
+// of it is NaN).
+__device__ __forceinline__ float mid_factor(int e) { return __int_as_float((267 - max(e, 13)) << 23); }
+__device__ __forceinline__ float mid_back(int e) { return e == 255 ? __int_as_float(0x7FC00000) : pow2(max(e, 13) - 140); }
 
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 // Largest magnitude (bits) of the lanes of a block: eight elements a lane.
@@ -260,7 +262,7 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) moe_few_route_kernel(const _
 #pragma unroll
     for (int w = 0; w < ROUTE_WARPS; ++w) top = max(top, s_top[w]);
     row_e = static_cast<int>(top >> 23);
-    if (tid == 0) p.x_factor[tok] = row_factor<KIND>(row_e);
+    if (tid == 0) p.x_factor[tok] = x_factor(row_e);
   }
   // (pieces is a multiple of 32 for FP4: whole warps take the shuffles)
   for (int c = tid; c < pieces; c += ROUTE_WARPS * 32) {
@@ -272,7 +274,9 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) moe_few_route_kernel(const _
       float v[8];
       unpack8(raw, v);
       uint32_t w[5];
-      const uint32_t sf = digits8<KIND>(v, block_top<KIND>(v), row_e, w);
+      uint32_t sf;
+      const float f = block_factor<KIND>(block_top<KIND>(v), row_e, sf);
+      digits8(v, f, w);
       uint8_t* img = p.x_img + static_cast<size_t>(kt) * p.n * 128;
       uint8_t* sfs = p.x_img + static_cast<size_t>(k_tiles) * p.n * 128 + static_cast<size_t>(kt) * T::SF_BYTES;
       const bool first = (c & (T::BLOCK / 8 - 1)) == 0;
@@ -466,7 +470,7 @@ __device__ __forceinline__ void tma_load_2d_once(uint32_t smem_dst, const CUtens
 __host__ __device__ constexpr int align_to(int v, int a) { return (v + a - 1) / a * a; }
 constexpr int BAR_BYTES = (3 * MAX_STAGES + 8) * 8;
 // Shared memory, from a 1024-byte boundary on: fc1: B tiles of x | stages | scales of x | candidates of the top-k | plan | barriers;
-// fc2: stages | sums [2][tokens][128] | plan | barriers
+// fc2: stages | sums [2][tokens][128] | scales of one | plan | barriers
 __host__ __device__ inline int k_tiles_of(int k, int tile) { return (k + tile - 1) / tile; }
 template <int KIND>
 __host__ __device__ inline int fc1_fixed_bytes(int tokens, int n, int hidden) {
@@ -475,11 +479,11 @@ __host__ __device__ inline int fc1_fixed_bytes(int tokens, int n, int hidden) {
 }
 template <int KIND>
 __host__ __device__ inline int fc2_fixed_bytes(int tokens) {
-  return 1024 + 2 * tokens * 512 + align_to(sizeof(Plan), 16) + BAR_BYTES;
+  return 1024 + 2 * tokens * 512 + 512 + align_to(sizeof(Plan), 16) + BAR_BYTES;
 }
-constexpr int ACC_COLS = 96;              // two accumulators, then scales of A and B (16 columns each)
+constexpr int ACC_COLS = 96;              // two accumulators, then scales of A (a tile's) and of B (all tiles' where they fit)
 constexpr int SFA_COL = 192, SFB_COL = 208;
-constexpr int TMEM_COLS = 256;
+constexpr int TMEM_COLS = 512;
 
 template <int KIND, bool SECOND>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -495,8 +499,8 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
   uint8_t* ring = sm + x_bytes;
   uint8_t* after = ring + S * STAGE;
   float* sums = reinterpret_cast<float*>(after);                                // fc2: [2][tokens][128]
-  uint8_t* xsf = after;                                                         // fc1
-  uint8_t* plan_at = after + (SECOND ? 2 * p.tokens * 512 : xsf_bytes + p.tokens * CAND_BYTES);
+  uint8_t* xsf = SECOND ? after + 2 * p.tokens * 512 : after;                   // scales of operand B
+  uint8_t* plan_at = after + (SECOND ? 2 * p.tokens * 512 + 512 : xsf_bytes + p.tokens * CAND_BYTES);
   Plan& plan = *reinterpret_cast<Plan*>(plan_at);
   uint64_t* full = reinterpret_cast<uint64_t*>(plan_at + align_to(sizeof(Plan), 16));
   uint64_t* empty = full + MAX_STAGES;
@@ -533,6 +537,8 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
   }
   if constexpr (SECOND) {
     for (int i = tid; i < 2 * p.tokens * 128; i += THREADS) sums[i] = 0.f;
+    if (tid < 128) reinterpret_cast<uint32_t*>(xsf)[tid] = KIND == kGemmMxfp4 ? 0x7F7F7F7Fu : 0x38383838u;
+    fence_proxy_async_smem();
   } else {
     (&plan.chosen[0][0])[tid] = 0;
   }
@@ -609,7 +615,7 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
   const int stride = SECOND ? __shfl_sync(0xffffffffu, static_cast<int>(cluster_n), 0) : static_cast<int>(gridDim.x);
   const int out_block = SECOND ? static_cast<int>(blockIdx.x) / stride : 0;
 
-  if constexpr (SECOND && KIND == kGemmNvfp4) {          // the largest exponent of every row this CTA reads
+  if constexpr (SECOND && T::kFp4) {          // the largest exponent of every row this CTA reads
     const int n_exp = ((p.swiglu ? 2 * p.inter : p.inter) + 31) / 32;
     for (int u = u0 + warp * stride; u < units; u += WARPS * stride)
       for (int c = 0; c < plan.count[u]; ++c) {
@@ -661,6 +667,16 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
     uint32_t phase = 0;
     bool ok = true, ready = false;
     if constexpr (!SECOND) ok = __all_sync(0xffffffffu, mbar_wait(x_full, 0, abort, p.status, kTimeoutFull));
+    // Scales of B that stay: fc2's are one; fc1's are every tile's, for as many columns as there are (a wider NVFP4 row copies them
+    // tile by tile). Each copy is 0.02 us of this warp's time per tile, which is what bounds a CTA that has its bytes.
+    const bool resident = SECOND || SFB_COL + k_tiles * T::ATOMS * 4 <= TMEM_COLS;
+    if constexpr (T::kFp4) {
+      tc_fence_after();
+      if (resident && ok && elect_one())
+        for (int at = 0; at < (SECOND ? 1 : k_tiles * T::ATOMS); ++at)
+          tmem_cp_32x128b_x4(tmem + SFB_COL + at * 4, make_desc_sf(xsf_addr + at * 512));
+      __syncwarp();
+    }
     for (int u = u0; u < units && ok; u += stride, ++it) {
       const int n = __shfl_sync(0xffffffffu, SECOND ? (plan.count[u] * P + 15) / 16 * 16 : p.n, 0);
       const uint32_t acc = tmem + (it & 1) * ACC_COLS;
@@ -682,16 +698,17 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
         // of the next tile, answered while this one is issued: a wait that finds its barrier complete takes 0.1 us all the same
         const bool peek = mbar_test_wait(&full[s], phase) && (!SECOND || mbar_test_wait(&b_full[s], phase));
         const uint32_t st = ring_addr + s_at * STAGE;
-        const uint32_t b_at = SECOND ? st + A_BYTES + T::SF_BYTES * 2 : ring_addr - x_bytes + kt * p.n * 128;
+        const uint32_t b_at = SECOND ? st + A_BYTES + T::SF_BYTES : ring_addr - x_bytes + kt * p.n * 128;
+        const uint32_t sfb = tmem + SFB_COL + (!SECOND && resident ? kt * T::ATOMS * 4 : 0);
         const uint64_t adesc = make_desc_sw128(st), bdesc = make_desc_sw128(b_at);
         const int mmas = min(4, (K - kt * T::TILE_K + T::MMA_K - 1) / T::MMA_K);
         if (elect_one()) {
           if constexpr (T::kFp4) {
-            const uint32_t sfb = SECOND ? st + A_BYTES + T::SF_BYTES : xsf_addr + kt * T::SF_BYTES;
 #pragma unroll
-            for (int at = 0; at < T::ATOMS; ++at) {
-              tmem_cp_32x128b_x4(tmem + SFA_COL + at * 4, make_desc_sf(st + A_BYTES + at * 512));
-              tmem_cp_32x128b_x4(tmem + SFB_COL + at * 4, make_desc_sf(sfb + at * 512));
+            for (int at = 0; at < T::ATOMS; ++at) tmem_cp_32x128b_x4(tmem + SFA_COL + at * 4, make_desc_sf(st + A_BYTES + at * 512));
+            if (!SECOND && !resident) {
+#pragma unroll
+              for (int at = 0; at < T::ATOMS; ++at) tmem_cp_32x128b_x4(sfb + at * 4, make_desc_sf(xsf_addr + kt * T::SF_BYTES + at * 512));
             }
           }
 #pragma unroll
@@ -700,10 +717,10 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
             const uint32_t more = kt > 0 || kb > 0 ? 1u : 0u;
             if constexpr (KIND == kGemmMxfp4)
               mma_mxf4(acc, adesc + kb * 2, bdesc + kb * 2, make_idesc_mxf4(128, 0, kb & 1) | static_cast<uint32_t>(n >> 3) << 17, more,
-                       tmem + SFA_COL + (kb >> 1) * 4, tmem + SFB_COL + (kb >> 1) * 4);
+                       tmem + SFA_COL + (kb >> 1) * 4, SECOND ? sfb : sfb + (kb >> 1) * 4);
             else if constexpr (KIND == kGemmNvfp4)
               mma_nvf4(acc, adesc + kb * 2, bdesc + kb * 2, make_idesc_nvf4(128, 0) | static_cast<uint32_t>(n >> 3) << 17, more,
-                       tmem + SFA_COL + kb * 4, tmem + SFB_COL + kb * 4);
+                       tmem + SFA_COL + kb * 4, SECOND ? sfb : sfb + kb * 4);
             else
               mma_f16(acc, adesc + kb * 2, bdesc + kb * 2, make_idesc_bf16(128, 0) | static_cast<uint32_t>(n >> 3) << 17, more);
           }
@@ -740,7 +757,7 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
 #pragma unroll
         for (int i = P - 2; i >= 0; --i) v = fmaf(v, T::kFp4 ? 8.f : 1.f, __uint_as_float(r[i]));
         if constexpr (SECOND) {
-          const float f = KIND == kGemmNvfp4 ? row_factor<KIND>(plan.row_exp[pr]) * gs : gs;
+          const float f = T::kFp4 ? mid_back(plan.row_exp[pr]) * gs : gs;
           sums[(set * p.tokens + tok) * 128 + row_in] += v * f * plan.weights[pr];
         } else {
           v *= KIND == kGemmNvfp4 ? ld_step(p.x_factor + tok) * gs : gs;
@@ -752,7 +769,7 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
           }
           const bool mine = row < rows_per_expert && (!p.swiglu || (lane & 1) == 0);
           if (mine) p.mid[static_cast<size_t>(pr) * p.inter + (p.swiglu ? row >> 1 : row)] = v;
-          if constexpr (KIND == kGemmNvfp4) {
+          if constexpr (T::kFp4) {
             const uint32_t m = __reduce_max_sync(0xffffffffu, mine ? magnitude(v) : 0u);
             if (lane == 0) p.mid_exp[static_cast<size_t>(pr) * p.exp_ld + tile * 4 + q] = static_cast<uint8_t>(m >> 23);
           }
@@ -778,8 +795,7 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
         next = CONVERTERS - 1;
         ok = __all_sync(0xffffffffu, mbar_wait(&empty[mine], turn, abort, p.status, kTimeoutEmpty));
         if (!ok) break;
-        uint8_t* sfb = ring + mine * STAGE + A_BYTES + T::SF_BYTES;
-        uint8_t* b = sfb + T::SF_BYTES;
+        uint8_t* b = ring + mine * STAGE + A_BYTES + T::SF_BYTES;
         if constexpr (T::kFp4) {
           const int k = kt * T::TILE_K + lane * 8;
 #pragma unroll 2
@@ -792,14 +808,9 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
               v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w; v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
             }
             uint32_t w[5];
-            const uint32_t sf = digits8<KIND>(v, block_top<KIND>(v), KIND == kGemmNvfp4 ? plan.row_exp[pr] : 0, w);
-            const bool first = (lane & (T::BLOCK / 8 - 1)) == 0;
+            digits8(v, mid_factor(plan.row_exp[pr]), w);
 #pragma unroll
-            for (int d = 0; d < 5; ++d) {
-              const int nr = c * 5 + d;
-              *reinterpret_cast<uint32_t*>(b + b_offset(nr, lane * 4)) = w[d];
-              if (first) sfb[sf_offset(nr, lane / (T::BLOCK / 8))] = static_cast<uint8_t>(sf);
-            }
+            for (int d = 0; d < 5; ++d) *reinterpret_cast<uint32_t*>(b + b_offset(c * 5 + d, lane * 4)) = w[d];
           }
         } else {
           for (int c = lane >> 3; c < n; c += 4) {
@@ -841,8 +852,16 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
     else __syncthreads();
     for (int i = tid + static_cast<int>(cluster_rank) * THREADS; i < n_out; i += THREADS * static_cast<int>(cluster_n)) {
       float s = 0.f;
-      const uint32_t at = smem_u32(sums + i);
-      for (uint32_t r = 0; r < cluster_n; ++r) s += cluster_n > 1 ? ld_dsmem_f32(map_to_cta(at, r)) : sums[i];
+      if (cluster_n > 1) {                  // all loads under way before the first sum
+        const uint32_t at = smem_u32(sums + i);
+        float part[MAX_CLUSTER];
+#pragma unroll
+        for (uint32_t r = 0; r < MAX_CLUSTER; ++r) part[r] = r < cluster_n ? ld_dsmem_f32(map_to_cta(at, r)) : 0.f;
+#pragma unroll
+        for (uint32_t r = 0; r < MAX_CLUSTER; ++r) s += part[r];
+      } else {
+        s = sums[i];
+      }
       const int tok = i >> 7, row = out_block * 128 + (i & 127);
       if (row < p.h_out) {
         if (p.shared != nullptr) s += __bfloat162float(p.shared[tok * p.ld_shared + row]);
