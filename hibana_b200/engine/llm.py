@@ -206,7 +206,7 @@ class LLM:
         depth = cfg.spec_depth + 1 if cfg.spec != "off" else 1
         tokens = max(cfg.prefill_budget, cfg.prefill_chunk or t.prefill_chunk, cfg.max_batch * depth)
         return ExpertParallel.create(rank, ep, self.device, tokens=tokens, topk=t.top_k, experts=t.experts,
-                                     hidden=width, fmt="nvfp4" if t.weight_format == "nvfp4" else "bf16",
+                                     hidden=width, fmt=t.weight_format if t.weight_format in ("nvfp4", "mxfp4") else "bf16",
                                      timeout_ms=cfg.comm_timeout_ms)
 
     def generate(self, prompts: Sequence[Sequence[int]],

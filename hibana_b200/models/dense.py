@@ -27,7 +27,7 @@ class DenseLayer:
         this rank's shard is cut out: q/k/v by head and gate/up by column (column-parallel), o_proj and down by
         input feature (row-parallel)."""
         h, d = t.hidden, t.head_dim
-        fmt = "nvfp4" if t.weight_format == "nvfp4" else "bf16"
+        fmt = t.weight_format if t.weight_format in ("nvfp4", "mxfp4") else "bf16"
 
         def rnd(n, k):
             return torch.randn(n, k, generator=gen, dtype=torch.float32, device=gen.device) * std
@@ -199,7 +199,8 @@ class DenseModel:
         """ids int64 [T]; kv = KvPool. Returns normed hidden states of ctx.sample_rows (or of all rows)."""
         t = self.target
         if (ctx.comm is not None and getattr(ctx.comm, "sp_rows", 0) and ctx.mode == "prefill"
-                and ctx.comm.sp_ok(ids.shape[0], t.hidden) and not self.layers[0].qkv.calibrating):
+                and ctx.comm.sp_ok(ids.shape[0], t.hidden) and not self.layers[0].qkv.calibrating
+                and self.layers[0].qkv.fmt != "mxfp4"):          # the peer-memory chain carries bf16 and NVFP4 rows
             return self.forward_sp(ids, ctx, kv)
         res = basic.embedding(ids, self.embed)
         if ctx.comm is None and self.layers[0].qkv.takes_gemv(ids.shape[0]) and self.layers[0].o.w3 is None:

@@ -122,13 +122,13 @@ class HybridModel:
         return out
 
     def attach_w3(self) -> int:
-        """3-bit decode copies (settings `w3`) of every NVFP4 / bf16 projection whose shape the 3-bit kernel tiles and
+        """3-bit decode copies (settings `w3`) of every FP4 / bf16 projection whose shape the 3-bit kernel tiles and
         of every MoE layer's routed experts: decode- and verify-sized calls stream 4 bits per weight, prefill keeps
         the served formats. Returns the bytes the copies add. Reference: hibana/kernels/w3.py `attach_model`."""
         from .linear import Linear
         added = 0
         for lin in self.linears():
-            if type(lin) is not Linear or lin.in_features % 64 or lin.fmt not in ("bf16", "nvfp4"):
+            if type(lin) is not Linear or lin.in_features % 64 or lin.fmt not in ("bf16", "nvfp4", "mxfp4"):
                 continue
             if lin.name.endswith(".router"):
                 continue            # fp32 logits: routing decisions stay those of the served weights

@@ -77,7 +77,7 @@ class Init:
 
 
 def _fmt(t: Target) -> str:
-    return "nvfp4" if t.weight_format == "nvfp4" else "q8_0" if t.weight_format == "ggml" else "bf16"
+    return t.weight_format if t.weight_format in ("nvfp4", "mxfp4") else "q8_0" if t.weight_format == "ggml" else "bf16"
 
 
 class AttentionLayer:
@@ -478,7 +478,7 @@ class MoeLayer:
         n1, n2 = ew.n1, ew.fc2_rows
         if n1 % 128 or n2 % 128 or ew.hidden % 64 or ew.inter % 64:
             return 0            # the 3-bit tiles cover 128 rows x 64 columns
-        dev = ew.fc1.q.device if ew.fmt == "nvfp4" else ew.fc1.device
+        dev = ew.fc1.q.device if ew.fmt in ("nvfp4", "mxfp4") else ew.fc1.device
         if fc1 is None:
             self.experts_w3 = moe.ExpertWeights.create(ew.dense(1), ew.dense(2), ew.act, "w3").to(dev)
         else:
@@ -501,8 +501,42 @@ class MoeLayer:
                                        scale=t.router_scale)
         return ids, w
 
+    def _takes_few(self, rows: int) -> bool:
+        """Whether a call of `rows` rows runs as one few-token layer (`moe.layer_forward`): MXFP4 experts always, the other
+        formats with `moe_few`. Off where the routing is edited between its kernels (`expert_budget`) and under
+        `stable_numerics` (the form reads unquantised activations, so a request's tokens would depend on how many rows ran
+        beside it)."""
+        cfg, ew = cfgmod.current(), self.experts
+        return (0 < rows <= moe.FEW_TOKENS and (ew.fmt == "mxfp4" or cfg.moe_few) and self.ep_size == 1
+                and self.experts_w3 is None and cfg.expert_budget <= 0 and not cfg.stable_numerics
+                and moe.few_tokens_ok(ew, self.t.top_k))
+
+    def _forward_few(self, x, ctx) -> torch.Tensor:
+        t = self.t
+        # (only a latent layer has something to run beside the shared expert: the sum of the others' joins in their last kernel)
+        with streams.Branch(x, enabled=bool(t.latent) and overlap_ok(x, ctx)) as br:
+            lat = self.fc1_latent(x) if t.latent else x
+            lat_ready = br.mark()
+            shared = self.shared.forward(x) if self.shared is not None else None
+            if shared is not None and self.shared_split and ctx is not None and ctx.comm is not None:
+                shared = ctx.comm.all_reduce(shared)
+        if t.latent:
+            br.wait(lat_ready, lat)
+        else:
+            br.join(shared)                   # the layer adds it in its last kernel
+        y = moe.layer_forward(lat, self.router.weight, self.experts, t.top_k, sigmoid=t.router == "sigmoid",
+                              sel_bias=self.sel_bias, renorm=True, scale=t.router_scale,
+                              shared=None if t.latent else shared, route_x=x if t.latent else None)
+        if not t.latent:
+            return y
+        out = self.fc2_latent(y)
+        br.join(shared)
+        return basic.add(out, shared) if shared is not None else out
+
     def forward(self, x, ctx=None, kv=None, states=None) -> torch.Tensor:
         t = self.t
+        if self._takes_few(x.shape[0]):
+            return self._forward_few(x, ctx)
         if overlap_ok(x, ctx):
             # decode-sized on one GPU: the latent projection and the shared expert do not depend on the routing, so
             # they run on a side stream beside router -> route -> plan -> grouped GEMMs (utils/streams.py)

@@ -1,4 +1,4 @@
-"""Linear layers over the quantised weight formats (bf16, NVFP4; w3 and FP8 plug in through the same interface).
+"""Linear layers over the quantised weight formats (bf16, NVFP4, MXFP4; w3 and FP8 plug in through the same interface).
 
 A `Linear` owns one weight matrix [N, K] in its storage format plus the static activation scale NVFP4 needs.
 `norm_linear` runs (residual add +) RMSNorm and the following projection with the norm fused into the
@@ -12,7 +12,8 @@ from typing import Optional, Union
 import torch
 
 from .. import config as cfgmod
-from ..ops import basic, gemm, gemv, nvfp4
+from ..ops import basic, gemm, gemv, mxfp4, nvfp4
+from ..ops.mxfp4 import Mxfp4Tensor
 from ..ops.nvfp4 import Nvfp4Tensor
 
 Activation = Union[torch.Tensor, Nvfp4Tensor]
@@ -29,7 +30,8 @@ def interleave_pairs(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
 
 
 class Linear:
-    """y = x @ W.T. `fmt` is 'bf16' or 'nvfp4'. `input_amax` is the calibrated activation range (NVFP4 only)."""
+    """y = x @ W.T. `fmt` is 'bf16', 'nvfp4' or 'mxfp4'. `input_amax` is the calibrated activation range (NVFP4 only:
+    the scales of MXFP4 activations come with their blocks)."""
 
     def __init__(self, weight: torch.Tensor, fmt: str = "bf16", input_amax: float = 8.0, name: str = ""):
         self.fmt = fmt
@@ -45,6 +47,9 @@ class Linear:
             self.wq = nvfp4.quantize_weight(weight)
             self.weight = None
             self.set_input_amax(input_amax)
+        elif fmt == "mxfp4":
+            self.wq = mxfp4.quantize_weight(weight)
+            self.weight = None
         else:
             raise ValueError(f"unknown linear format {fmt!r}")
 
@@ -53,10 +58,14 @@ class Linear:
                 name: str = "") -> "Linear":
         """A tensor-parallel shard that is bitwise a slice of the unsharded layer: the full matrix is quantised
         with its own per-tensor scale and then rows (output features) and / or columns (input features, on
-        16-element block boundaries) are cut out. Reference: hibana/weights/sharding.py:15-19,
+        16-element block boundaries, 32 for MXFP4) are cut out. Reference: hibana/weights/sharding.py:15-19,
         hibana/model/flashnext/linear.py:31-43."""
         rows = slice(None) if rows is None else rows
         cols = slice(None) if cols is None else cols
+        if fmt == "mxfp4":
+            full = mxfp4.quantize_weight(weight)
+            c0, c1 = cols.start or 0, cols.stop if cols.stop is not None else full.k
+            return cls.from_mxfp4(mxfp4.from_blocks(*mxfp4.cut(full.q, full.scales(), rows, c0, c1)), name=name)
         if fmt != "nvfp4":
             return cls(weight[rows][:, cols], fmt, name=name)
         full = nvfp4.quantize_weight(weight)
@@ -81,6 +90,15 @@ class Linear:
         self.alpha = (self.input_scale * wq.gscale).reshape(1)
         return self
 
+    @classmethod
+    def from_mxfp4(cls, wq: Mxfp4Tensor, name: str = "") -> "Linear":
+        """Wraps an MXFP4 matrix (see `mxfp4.from_blocks` for a checkpoint's tensors)."""
+        self = cls.__new__(cls)
+        self.fmt, self.name, self.wq, self.weight = "mxfp4", name, wq, None
+        self.out_features, self.in_features = wq.rows, wq.k
+        self.calibrating, self.seen_amax, self.w3 = False, 0.0, None
+        return self
+
     def set_input_amax(self, amax: float) -> None:
         dev = self.wq.q.device
         self.input_scale = torch.tensor([max(amax, 1e-6) / (6.0 * 448.0)], dtype=torch.float32, device=dev)
@@ -89,7 +107,9 @@ class Linear:
     def to(self, device) -> "Linear":
         if self.weight is not None:
             self.weight = self.weight.to(device)
-        if self.wq is not None:
+        if self.fmt == "mxfp4":
+            self.wq = self.wq.to(device)
+        elif self.wq is not None:
             w = self.wq
             self.wq = Nvfp4Tensor(w.q.to(device), w.sf.to(device), w.gscale.to(device), w.rows, w.k)
             self.input_scale = self.input_scale.to(device)
@@ -150,6 +170,9 @@ class Linear:
         if (not isinstance(x, Nvfp4Tensor) and epilogue in (gemm.EPI_STORE, gemm.EPI_RESIDUAL, gemm.EPI_SILU_MUL)
                 and self.takes_gemv(x.shape[0])):
             y = gemv.nvfp4_gemv(x, self.wq, epilogue=epilogue, residual=residual, out=out, static_weight=True)
+            return y if requant is None else nvfp4.quantize(y, requant)
+        if self.fmt == "mxfp4":
+            y = gemm.linear_mxfp4(mxfp4.quantize(x), self.wq, epilogue=epilogue, residual=residual, out=out, static_weight=True)
             return y if requant is None else nvfp4.quantize(y, requant)
         xq = x if isinstance(x, Nvfp4Tensor) else self.quantize_input(x)
         if requant is not None and epilogue == gemm.EPI_SILU_MUL:

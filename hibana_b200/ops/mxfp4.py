@@ -101,6 +101,14 @@ def from_blocks(packed: torch.Tensor, scales: torch.Tensor) -> Mxfp4Tensor:
     return Mxfp4Tensor(packed, swizzle_blocks(scales, k_atoms(k)), rows, k)
 
 
+def cut(packed: torch.Tensor, scales: torch.Tensor, rows, c0: int, c1: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows (slice or index tensor) and columns c0 .. c1 (whole blocks) of a matrix in row-major blocks; nothing is
+    requantised."""
+    if c0 % BLOCK or c1 % BLOCK:
+        raise ValueError(f"MXFP4: columns [{c0}, {c1}) are not whole blocks of {BLOCK}")
+    return packed[rows][:, c0 // 2:c1 // 2], scales[rows][:, c0 // BLOCK:c1 // BLOCK]
+
+
 def _check(x: torch.Tensor) -> None:
     if x.dim() != 2 or x.dtype not in IN_TYPES:
         raise ValueError(f"MXFP4: a bf16, fp16 or fp32 matrix expected, got {x.dtype} {tuple(x.shape)}")

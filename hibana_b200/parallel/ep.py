@@ -87,6 +87,9 @@ class ExpertParallel:
                timeout_ms: int = 2000, group=None) -> "ExpertParallel":
         """`tokens` bounds the tokens of one rank per call; `rows_cap` the rows one rank can receive (default: the
         worst case, every pair of every rank)."""
+        if fmt not in ("bf16", "nvfp4"):
+            raise ValueError(f"all-to-all expert parallelism carries bf16 or NVFP4 rows, not {fmt} (replicated activations do: "
+                             "dp = 1)")
         assert experts % world == 0 and world <= 8
         lib = nv.lib()
         torch.cuda.set_device(device)

@@ -58,7 +58,7 @@ class Target:
     mtp_layers: int = 0
     mtp_depth: int = 0
     # numerics / formats
-    weight_format: str = "bf16"      # bf16 | nvfp4 | w3
+    weight_format: str = "bf16"      # bf16 | nvfp4 | mxfp4 | w3
     kv_dtype: str = "bf16"           # bf16 | fp8
     norm_eps: float = 1e-6
     max_context: int = 262144

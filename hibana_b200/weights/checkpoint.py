@@ -27,6 +27,8 @@ INDEX = "model.safetensors.index.json"
 def _lin_tensors(lin: Linear, name: str) -> dict:
     if lin.fmt == "nvfp4":
         return modelopt.nvfp4_tensors(lin, name)
+    if lin.fmt == "mxfp4":
+        return modelopt.mxfp4_tensors(lin, name)
     return {f"{name}.weight": lin.weight.cpu().contiguous()}
 
 
@@ -41,6 +43,11 @@ def _split_rows(lin: Linear, name_rows: list, deinterleave: bool = False) -> dic
             out[f"{name}.weight_scale"] = base["x.weight_scale"].view(torch.uint8)[sel].contiguous().view(torch.float8_e4m3fn)
             out[f"{name}.weight_scale_2"] = base["x.weight_scale_2"].clone()
             out[f"{name}.input_scale"] = base["x.input_scale"].clone()
+    elif lin.fmt == "mxfp4":
+        base = modelopt.mxfp4_tensors(lin, "x")
+        for name, sel in name_rows:
+            out[f"{name}.weight"] = base["x.weight"][sel].contiguous()
+            out[f"{name}.weight_scale"] = base["x.weight_scale"][sel].contiguous()
     else:
         for name, sel in name_rows:
             out[f"{name}.weight"] = lin.weight.cpu()[sel].contiguous()
@@ -105,6 +112,8 @@ class Snapshot:
 
 
 def _load_lin(snap: Snapshot, name: str, device, rows=None, cols=None) -> Linear:
+    if modelopt.is_mxfp4(snap, name):
+        return Linear.from_mxfp4(modelopt.load_mxfp4(snap, [name], parts=[rows], cols=cols), name=name).to(device)
     if f"{name}.weight_scale" in snap:
         return modelopt.load_nvfp4_linear(snap, name, device, rows=rows, cols=cols)
     w = snap[f"{name}.weight"]
@@ -117,6 +126,9 @@ def _load_lin(snap: Snapshot, name: str, device, rows=None, cols=None) -> Linear
 
 def _load_fused(snap: Snapshot, names: list, device, parts=None, interleave: bool = False, name: str = "") -> Linear:
     """Separate stored projections -> one Linear (see modelopt.load_nvfp4_fused); bf16 sources are concatenated."""
+    if all(modelopt.is_mxfp4(snap, n) for n in names):
+        wq = modelopt.load_mxfp4(snap, names, parts=parts, interleave=interleave)
+        return Linear.from_mxfp4(wq, name=name or names[0]).to(device)
     if f"{names[0]}.weight_scale" in snap:
         return modelopt.load_nvfp4_fused(snap, names, device, parts=parts, interleave=interleave, name=name)
     ws = []

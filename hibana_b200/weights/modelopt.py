@@ -13,7 +13,7 @@ from typing import Mapping
 import torch
 
 from ..models.linear import Linear
-from ..ops import nvfp4
+from ..ops import mxfp4, nvfp4
 from ..ops.fp8 import Fp8Weight
 
 
@@ -81,6 +81,36 @@ def load_nvfp4_fused(tensors: Mapping[str, torch.Tensor], names: list, device="c
     wq = nvfp4.Nvfp4Tensor(q.contiguous().to(device), nvfp4.swizzle_sf(sf.contiguous()).to(device), gs.to(device),
                            n_rows, k)
     return Linear.from_nvfp4(wq, torch.stack(ins).max().reshape(1).to(device), name=name or names[0])
+
+
+def mxfp4_tensors(lin: Linear, name: str) -> dict:
+    """The two checkpoint tensors of an MXFP4 linear: packed values and row-major scale bytes (both uint8)."""
+    return {f"{name}.weight": lin.wq.q.cpu().contiguous(), f"{name}.weight_scale": lin.wq.scales().cpu().contiguous()}
+
+
+def is_mxfp4(tensors: Mapping[str, torch.Tensor], name: str) -> bool:
+    """Whether a stored projection is in MXFP4: scale bytes and no per-tensor scale."""
+    return (f"{name}.weight_scale" in tensors and f"{name}.weight_scale_2" not in tensors
+            and tensors[f"{name}.weight_scale"].dtype == torch.uint8)
+
+
+def load_mxfp4(tensors: Mapping[str, torch.Tensor], names: list, *, parts=None, interleave: bool = False,
+               cols=None) -> mxfp4.Mxfp4Tensor:
+    """One MXFP4 matrix out of one or several stored projections (see `load_nvfp4_fused`; blocks carry their own scales, so
+    any projections can be joined). `cols` are elements, a multiple of 32. Nothing is requantised."""
+    qs, sfs = [], []
+    for i, n in enumerate(names):
+        q, sf = tensors[f"{n}.weight"], tensors[f"{n}.weight_scale"]
+        sel = slice(None) if parts is None or parts[i] is None else parts[i]
+        c0, c1 = (0, 2 * q.shape[1]) if cols is None else (cols.start or 0, cols.stop)
+        q, sf = mxfp4.cut(q, sf, sel, c0, c1)
+        qs.append(q)
+        sfs.append(sf)
+    if interleave:
+        if len(qs) != 2 or qs[0].shape != qs[1].shape:
+            raise ValueError(f"{names}: two projections of one shape are interleaved")
+        return mxfp4.from_blocks(*(torch.stack(v, dim=1).flatten(0, 1) for v in (qs, sfs)))
+    return mxfp4.from_blocks(torch.cat(qs, 0), torch.cat(sfs, 0))
 
 
 def fp8_tensors(w: Fp8Weight, input_scale: torch.Tensor, name: str) -> dict:

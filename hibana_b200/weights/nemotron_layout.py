@@ -22,7 +22,7 @@ from safetensors.torch import save_file
 
 from ..models.linear import Linear
 from ..ops import moe as moe_ops
-from ..ops import nvfp4
+from ..ops import mxfp4, nvfp4
 from ..target import ATTN, GATED_ATTN, LATENT_MOE, MAMBA2, MOE, Target
 from . import modelopt
 from .checkpoint import INDEX, Snapshot, _lin_tensors, _load_fused, _load_lin, _split_rows
@@ -34,10 +34,12 @@ BACKBONE = f"{PREFIX}.backbone"
 def _expert_tensors(ew: moe_ops.ExpertWeights, which: int, e: int, name: str) -> dict:
     """Checkpoint tensors of expert `e`'s fc1 (which = 1) or fc2 matrix."""
     w = ew.fc1 if which == 1 else ew.fc2
-    rows = ew.n1 if which == 1 else (w.rows if ew.fmt == "nvfp4" else w.shape[0]) // ew.experts
+    rows = ew.n1 if which == 1 else ew.fc2_rows
     sel = slice(e * rows, (e + 1) * rows)
     if ew.fmt == "bf16":
         return {f"{name}.weight": w[sel].cpu().contiguous()}
+    if ew.fmt == "mxfp4":
+        return {f"{name}.weight": w.q[sel].cpu().contiguous(), f"{name}.weight_scale": w.scales()[sel].cpu().contiguous()}
     sf = nvfp4.unswizzle_sf(w.sf, w.rows, w.k // 16)
     in_scale = ew.fc1_in_scale if which == 1 else ew.fc2_in_scale
     return {f"{name}.weight": w.q[sel].cpu().contiguous(),
@@ -124,6 +126,11 @@ def _load_experts(snap: Snapshot, prefix: str, t: Target, device) -> moe_ops.Exp
         fc1 = torch.stack([snap[f"{n}.weight"] for n in names1])
         fc2 = torch.stack([snap[f"{n}.weight"] for n in names2])
         return moe_ops.ExpertWeights.create(fc1, fc2, t.moe_act, "bf16").to(device)
+    if modelopt.is_mxfp4(snap, names1[0]):
+        m1, m2 = modelopt.load_mxfp4(snap, names1), modelopt.load_mxfp4(snap, names2)
+        if m1.k != width:
+            raise ValueError(f"{prefix}: expert input width {m1.k} != {width}")
+        return moe_ops.ExpertWeights(t.experts, width, m2.k, t.moe_act, "mxfp4", m1, m2).to(device)
 
     def stack(names):
         q = torch.cat([snap[f"{n}.weight"] for n in names], 0)
