@@ -1006,13 +1006,13 @@ cudaError_t launch_t(const GemmArgs& a, DevParams& p, dim3 grid, const CUtensorM
                      cudaStream_t stream) {
   using C = Cfg<KIND, BN>;
   constexpr int K_ELEMS = is_fp4(KIND) ? 256 : KIND == kGemmFp8 ? 128 : 64;      // of a K tile
-  static bool attr_done = false;
+  static bool attr_done[kMaxDevices] = {};
   static int max_clusters[9] = {0, 0, 0, 0, 0, 0, 0, 0, 0};   // co-resident clusters per cluster size (0 = unknown)
-  if (!attr_done) {
+  if (bool& done = attr_done[device_index()]; !done) {
     cudaError_t e = cudaFuncSetAttribute(gemm_kernel<KIND, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          C::SMEM_BYTES);
     if (e != cudaSuccess) return e;
-    attr_done = true;
+    done = true;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(NUM_THREADS);

@@ -642,7 +642,7 @@ bool gemm_pair_ok(const GemmArgs& a) {
 }
 
 cudaError_t gemm_pair_launch(const GemmArgs& a, cudaStream_t stream) {
-  static const int resident_nv = [] {
+  const auto resident_nv = [] {
     int n = resident_clusters<kGemmNvfp4, kEpiStore, false>();
     n = std::min(n, resident_clusters<kGemmNvfp4, kEpiResidual, false>());
     n = std::min(n, resident_clusters<kGemmNvfp4, kEpiSiluMul, false>());
@@ -650,14 +650,17 @@ cudaError_t gemm_pair_launch(const GemmArgs& a, cudaStream_t stream) {
     n = std::min(n, resident_clusters<kGemmNvfp4, kEpiStore, true>());
     n = std::min(n, resident_clusters<kGemmNvfp4, kEpiRelu2Quant, true>());
     return std::min(n, resident_clusters<kGemmNvfp4, kEpiSiluMulQuant, true>());
-  }();
-  static const int resident_mx = [] {
+  };
+  const auto resident_mx = [] {
     int n = resident_clusters<kGemmMxfp4, kEpiStore, false>();
     n = std::min(n, resident_clusters<kGemmMxfp4, kEpiResidual, false>());
     return std::min(n, resident_clusters<kGemmMxfp4, kEpiSiluMul, false>());
-  }();
+  };
   const bool mx = a.kind == kGemmMxfp4;
-  const int resident = mx ? resident_mx : resident_nv;
+  static int known[2][kMaxDevices] = {};      // + 1
+  int& slot = known[mx][device_index()];
+  if (slot == 0) slot = (mx ? resident_mx() : resident_nv()) + 1;
+  const int resident = slot - 1;
   if (resident < 1) return cudaErrorInvalidConfiguration;
   const bool grouped = a.grp_cnt != nullptr;
   // tokens are the A side here; a grouped call names its weights first

@@ -14,6 +14,13 @@
 
 namespace hb {
 
+constexpr int kMaxDevices = 16;   // of a process: kernel attributes are set once on each
+
+// Current device, as the index of such a table.
+inline int device_index() {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < kMaxDevices ? dev : kMaxDevices - 1;
+}
 constexpr int kNumSms = 148;      // two dies of 74 (hardware/b200.py NUM_SMS)
 
 // Status codes written to the status word (first writer wins; 0 = OK).

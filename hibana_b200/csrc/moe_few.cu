@@ -616,13 +616,15 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
   const int out_block = SECOND ? static_cast<int>(blockIdx.x) / stride : 0;
 
   if constexpr (SECOND && T::kFp4) {          // the largest exponent of every row this CTA reads
-    const int n_exp = ((p.swiglu ? 2 * p.inter : p.inter) + 31) / 32;
+    const int words = (p.swiglu ? 2 * p.inter : p.inter) / 128;      // of four exponents
     for (int u = u0 + warp * stride; u < units; u += WARPS * stride)
       for (int c = 0; c < plan.count[u]; ++c) {
         const int pr = plan.pair[u * COLS + c];
         uint32_t m = 0;
-        for (int i = lane; i < n_exp; i += 32) m = max(m, static_cast<uint32_t>(p.mid_exp[static_cast<size_t>(pr) * p.exp_ld + i]));
-        m = __reduce_max_sync(0xffffffffu, m);
+        for (int i = lane; i < words; i += 32)
+          m = __vmaxu4(m, ld_step(reinterpret_cast<const uint32_t*>(p.mid_exp + static_cast<size_t>(pr) * p.exp_ld) + i));
+        m = __vmaxu4(m, m >> 16);
+        m = __reduce_max_sync(0xffffffffu, max(m & 255u, (m >> 8) & 255u));
         if (lane == 0) plan.row_exp[pr] = static_cast<int>(m);
       }
     __syncthreads();
@@ -937,13 +939,14 @@ cudaError_t launch_few(FewParams& p, const void* w1, const void* w2, uint8_t* ws
   using T = Traits<KIND>;
   auto k1 = moe_few_experts_kernel<KIND, false>;
   auto k2 = moe_few_experts_kernel<KIND, true>;
-  static const cudaError_t ready = [&] {
+  static bool ready[kMaxDevices] = {};
+  if (bool& done = ready[device_index()]; !done) {
     cudaError_t e = cudaFuncSetAttribute(k1, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SMEM);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k2, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SMEM);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k2, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    return e;
-  }();
-  if (ready != cudaSuccess) return ready;
+    if (e != cudaSuccess) return e;
+    done = true;
+  }
   const WsLayout w = ws_layout<KIND>(p.tokens, p.experts, p.topk, p.hidden, p.inter);
   p.x_img = ws + w.img;
   p.mid = reinterpret_cast<float*>(ws + w.mid);

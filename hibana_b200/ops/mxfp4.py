@@ -135,6 +135,14 @@ def quantize(x: torch.Tensor, *, src_rows: torch.Tensor | None = None, total_row
     _check(x)
     m, k = x.shape
     m = m if rows is None else rows
+    if src_rows is None and (gather or total_rows is not None or m != x.shape[0]):
+        raise ValueError("MXFP4: gather, total_rows and rows go with src_rows")
+    if src_rows is not None:
+        if not x.is_cuda or not 0 <= m <= src_rows.numel() or (not gather and m > x.shape[0]):
+            raise ValueError(f"MXFP4: {m} rows of {x.shape[0]} by {src_rows.numel()} row numbers on {x.device}")
+        for v in (src_rows, total_rows):
+            if v is not None and (v.dtype != torch.int32 or v.device != x.device or not v.is_contiguous() or v.numel() < 1):
+                raise ValueError("MXFP4: row numbers and counts are contiguous int32 tensors on the rows' device")
     if nv.use_native(x):
         q, sf = _alloc(m, k, x.device)
         if m:

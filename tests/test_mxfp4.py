@@ -252,3 +252,23 @@ def test_product_in_a_graph_and_on_another_stream_gpu():
         static.copy_(r)
         g.replay()
         assert torch.equal(out, gemm.linear_mxfp4(mxfp4.quantize(r), w))
+
+
+def test_row_number_refusals_cpu():
+    x = torch.randn(4, 64).bfloat16()
+    idx = torch.arange(4, dtype=torch.int32)
+    for kw in ({"gather": True}, {"rows": 5}, {"total_rows": idx[:1]}, {"src_rows": idx}):      # (row numbers are for the GPU)
+        with pytest.raises(ValueError):
+            mxfp4.quantize(x, **kw)
+
+
+@pytest.mark.gpu
+def test_row_number_refusals_gpu():
+    x = torch.randn(4, 64, device="cuda").bfloat16()
+    idx = torch.arange(8, dtype=torch.int32, device="cuda")
+    for kw in ({"src_rows": idx.long()}, {"src_rows": idx.cpu()}, {"src_rows": idx[::2]}, {"src_rows": idx, "rows": 5},
+               {"src_rows": idx, "rows": 9, "gather": True}, {"src_rows": idx, "total_rows": idx[:1].long()}):
+        with pytest.raises(ValueError):
+            mxfp4.quantize(x, **kw)
+    q = mxfp4.quantize(x, src_rows=idx.flip(0)[4:].contiguous(), rows=4, gather=True)
+    assert torch.equal(q.dequantize(), mxfp4.quantize(x.flip(0).contiguous()).dequantize())
