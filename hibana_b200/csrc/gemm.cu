@@ -1142,8 +1142,9 @@ cudaError_t gemm_launch(const GemmArgs& a, cudaStream_t stream) {
   if (fp4 && grouped && a.bn < 128 && a.grp_chunks != 1) return cudaErrorInvalidValue;
   const int atoms = k_tiles * sf_atoms(a.kind);
   if (fp4 && (a.sf_k_atoms_a < atoms || a.sf_k_atoms_b < atoms)) return cudaErrorInvalidValue;
-  // the requantising epilogues write NVFP4 for an NVFP4 product
-  if (a.kind == kGemmMxfp4 && (a.epilogue == kEpiSiluMulQuant || a.epilogue == kEpiRelu2Quant || a.peer != nullptr || a.ep != nullptr))
+  // (MXFP4 requantises in grouped calls only)
+  if (a.kind == kGemmMxfp4 && ((!grouped && (a.epilogue == kEpiSiluMulQuant || a.epilogue == kEpiRelu2Quant)) || a.peer != nullptr ||
+                               a.ep != nullptr))
     return cudaErrorInvalidValue;
   int splits = a.splits == 0 || grouped ? 1 : std::abs(a.splits);      // negative: see launch_t
   if (splits > k_tiles) splits = k_tiles;
@@ -1154,7 +1155,8 @@ cudaError_t gemm_launch(const GemmArgs& a, cudaStream_t stream) {
   if (grouped && (a.epilogue == kEpiSiluMulQuant || a.epilogue == kEpiRelu2Quant)) {
     // SM pairs only: whole 64-feature spans, every row's packed bytes on 16-byte boundaries
     const int feats = a.epilogue == kEpiSiluMulQuant ? a.grp_rows_a / 2 : a.grp_rows_a;
-    if (a.q_out == nullptr || a.q_sf == nullptr || a.q_gscale == nullptr || feats % 64 != 0 || a.q_ka * 64 < feats ||
+    const bool mx = a.kind == kGemmMxfp4;
+    if (a.q_out == nullptr || a.q_sf == nullptr || (a.q_gscale == nullptr) != mx || feats % 64 != 0 || a.q_ka * (mx ? 128 : 64) < feats ||
         a.q_ld % 16 != 0 || (reinterpret_cast<uintptr_t>(a.q_out) & 15) != 0 || !gemm_pair_ok(a))
       return cudaErrorInvalidValue;
   } else if (a.epilogue == kEpiRelu2Quant) {
@@ -1375,15 +1377,16 @@ int hb_gemm_grouped(int kind, const void* a, const void* b, const void* sfa, con
   return e == cudaSuccess ? 0 : static_cast<int>(e);
 }
 
-// The same with the activation (epilogue 7: SiLU-mul of interleaved gate / up rows, 8: squared ReLU) requantised to NVFP4 in
-// the epilogue: q_out [b_rows, q_ld bytes] and q_sf (q_ka K atoms per row block) are the activation operand of the next
+// The same in FP4 (kind 1: NVFP4, 4: MXFP4, which has no q_gscale and no alpha) with the activation (epilogue 7: SiLU-mul of
+// interleaved gate / up rows, 8: squared ReLU) requantised to the same format in the epilogue: q_out [b_rows, q_ld bytes] and q_sf (q_ka K atoms per row block) are the activation operand of the next
 // grouped call over the same rows. Needs the plan's work list for 256-row chunks (`tiles`).
-int hb_gemm_grouped_quant(const void* a, const void* b, const void* sfa, const void* sfb, int experts, int n_per_expert,
+int hb_gemm_grouped_quant(int kind, const void* a, const void* b, const void* sfa, const void* sfb, int experts, int n_per_expert,
                           int b_rows, int k, const void* alpha_ptr, int epilogue, const void* start, const void* cnt,
                           void* status, int ka_a, int ka_b, const void* tiles, const void* n_tiles, int tile_cap,
                           void* q_out, void* q_sf, const void* q_gscale, int q_ka, long long q_ld, void* stream) {
   hb::GemmArgs g;
-  g.kind = hb::kGemmNvfp4; g.a = a; g.b = b; g.sfa = sfa; g.sfb = sfb;
+  if (!hb::is_fp4(kind)) return 1;
+  g.kind = kind; g.a = a; g.b = b; g.sfa = sfa; g.sfb = sfb;
   g.ra = experts * n_per_expert; g.rb = b_rows; g.k = k; g.lda = k; g.ldb = k;
   g.out = nullptr; g.ldo = 0; g.residual = nullptr; g.alpha = 1.f;
   g.alpha_ptr = static_cast<const float*>(alpha_ptr); g.epilogue = epilogue; g.swap = 1; g.splits = 1;

@@ -32,8 +32,9 @@ enum GemmEpilogue : int {
   kEpiSiluMulQuant = 7,  // SiLU-mul as in kEpiSiluMul, then requantised to NVFP4 in the same epilogue: packed e2m1
                          // rows go to q_out, ue4m3 scales to q_sf (128x4-swizzled blocks) with the static per-tensor
                          // scale *q_gscale of the consuming projection. Weights on the 128-row side only; the next
-                         // GEMM reads the result as its activation operand with no kernel in between.
-  kEpiRelu2Quant = 8,    // squared ReLU as in kEpiRelu2, requantised to NVFP4 the same way (grouped calls on SM pairs)
+                         // GEMM reads the result as its activation operand with no kernel in between. Grouped MXFP4 calls
+                         // write MXFP4 (no per-tensor scale).
+  kEpiRelu2Quant = 8,    // squared ReLU as in kEpiRelu2, requantised the same way (grouped calls on SM pairs)
 };
 
 // Peer-memory fusion arguments (all ranks pass the same offsets; pointers are this process's mappings).

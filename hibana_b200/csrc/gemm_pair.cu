@@ -226,7 +226,7 @@ __device__ __forceinline__ float silu_fast(float x) { return __fdividef(x, 1.f +
 // One epilogue warp's part of a unit: 32 rows x half of its columns, in steps of 32 columns (one tcgen05.ld), two steps in
 // registers at a time. `acc` is the accumulator's address for the warp's lanes, `release` the leader's acc_free barrier.
 // The columns that the two accumulators share come first: the last ones of the first, the first ones of the second.
-template <int EPI, bool GRP>
+template <int KIND, int EPI, bool GRP>
 __device__ __forceinline__ void epilogue_unit(const PairParams& p, const Unit& x, int buf, int half, uint32_t acc, int row0,
                                               uint8_t* staging, float alpha, float q_inv_gs, uint32_t release, int lane) {
   if (GRP && row0 >= x.m_end) {                     // none of these rows is stored (the segment's padding)
@@ -250,7 +250,39 @@ __device__ __forceinline__ void epilogue_unit(const PairParams& p, const Unit& x
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(release);
     }
-    if constexpr (EPI == kEpiSiluMulQuant || EPI == kEpiRelu2Quant) {
+    if constexpr (KIND == kGemmMxfp4 && (EPI == kEpiSiluMulQuant || EPI == kEpiRelu2Quant)) {
+      // Two steps (grouped units have no odd one) are 32 or 64 features of the thread's token: one or two blocks.
+      static_assert(GRP, "widths of 128 and 256");
+      constexpr int BLOCKS = EPI == kEpiSiluMulQuant ? 1 : 2;
+      constexpr int SHIFT = EPI == kEpiSiluMulQuant ? 6 : 5;      // columns per block, log2
+      const int c = x.n0 + col0 + s0 * 32;
+      uint4 pk[BLOCKS];
+      uint32_t sfw = 0;
+#pragma unroll
+      for (int g = 0; g < BLOCKS; ++g) {
+        float y[32];
+#pragma unroll
+        for (int t = 0; t < 32; ++t) {              // rounded as a bf16 store would
+          float v;
+          if constexpr (EPI == kEpiSiluMulQuant) {
+            v = silu_fast(__uint_as_float(r[t >> 4][2 * t & 31]) * alpha) * (__uint_as_float(r[t >> 4][(2 * t & 31) + 1]) * alpha);
+          } else {
+            v = __uint_as_float(r[g][t]) * alpha;
+            v = v <= 0.f ? 0.f : v * v;             // (a NaN stays one)
+          }
+          y[t] = __bfloat162float(__float2bfloat16(v));
+        }
+        sfw |= quant32_mx(y, pk[g]) << (8 * g);
+      }
+      if (row < x.m_end && c < p.n) {               // (columns come in 128)
+        uint8_t* dst = p.q_out + static_cast<size_t>(row) * p.q_ld + (c >> SHIFT) * 16;
+        uint8_t* sf = p.q_sf + row_sf_off(row, c >> SHIFT, p.q_ka);
+#pragma unroll
+        for (int g = 0; g < BLOCKS; ++g) *reinterpret_cast<uint4*>(dst + g * 16) = pk[g];
+        if constexpr (BLOCKS == 2) *reinterpret_cast<uint16_t*>(sf) = static_cast<uint16_t>(sfw);
+        else sf[0] = static_cast<uint8_t>(sfw);
+      }
+    } else if constexpr (EPI == kEpiSiluMulQuant || EPI == kEpiRelu2Quant) {
       // The thread's token: two steps are 32 or 64 features, 16 or 32 packed bytes and two or four scale bytes, which go straight
       // from registers to whole or half sectors. Same arithmetic in the same order as the stand-alone quantiser. Whole steps are
       // in range or none: ungrouped SiLU-mul calls have a multiple of 64 gate and up columns, grouped calls of 64 features.
@@ -349,7 +381,7 @@ __device__ __forceinline__ void epilogue_unit(const PairParams& p, const Unit& x
     }
   }
   if constexpr (EPI == kEpiSiluMulQuant || EPI == kEpiRelu2Quant) {
-    constexpr int SHIFT = EPI == kEpiSiluMulQuant ? 5 : 4;
+    constexpr int SHIFT = (EPI == kEpiSiluMulQuant ? 5 : 4) + (KIND == kGemmMxfp4 ? 1 : 0);
     if (row < x.m_end && half == 1 && x.n0 + x.width >= p.n)      // groups that pad the last K tile of the next GEMM read as zero
       for (int w = p.n >> SHIFT; w < p.q_ka * 4; ++w) p.q_sf[row_sf_off(row, w, p.q_ka)] = 0;
   }
@@ -557,7 +589,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__
     uint8_t* mine = staging + (warp - 2) * 32 * ROW_PITCH;
     float alpha = p.alpha;
     if (!GRP && p.alpha_ptr != nullptr) alpha *= *p.alpha_ptr;
-    const float q_inv_gs = EPI == kEpiSiluMulQuant || EPI == kEpiRelu2Quant ? 1.f / *p.q_gscale : 0.f;
+    const float q_inv_gs = KIND == kGemmNvfp4 && (EPI == kEpiSiluMulQuant || EPI == kEpiRelu2Quant) ? 1.f / *p.q_gscale : 0.f;
     int it = 0;
     for (UnitWalk<GRP> w(p, cluster, clusters); w.more(); w.next()) {
       const Unit x = w.unit();
@@ -567,7 +599,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__
       // one verdict per warp: lanes that give up on a wait must not leave the others alone in a warp-wide TMEM load
       if (!__all_sync(0xffffffffu, mbar_wait(&accum[buf], (it >> 1) & 1, abort, p.status, kTimeoutAccum))) break;
       tc_fence_after();
-      epilogue_unit<EPI, GRP>(p, x, buf, half, tlane + (buf ? ACC1_COL : 0), x.m0 + static_cast<int>(rank) * 128 + q * 32, mine,
+      epilogue_unit<KIND, EPI, GRP>(p, x, buf, half, tlane + (buf ? ACC1_COL : 0), x.m0 + static_cast<int>(rank) * 128 + q * 32, mine,
                          alpha, q_inv_gs, release, lane);
       ++it;
     }
@@ -626,13 +658,12 @@ int resident_clusters() {
 bool gemm_pair_ok(const GemmArgs& a) {
   if (!is_fp4(a.kind) || a.peer != nullptr || a.ep != nullptr || a.tok_scale != nullptr || a.bn != 256) return false;
   const bool grouped = a.grp_cnt != nullptr;
-  if (a.kind == kGemmMxfp4 && grouped) return false;
   if (grouped) {
     if (!a.swap || a.grp_tiles == nullptr || a.grp_rows_a % 128 != 0) return false;
   } else if (a.swap || a.splits > 1) {
     return false;
   }
-  if (a.epilogue == kEpiSiluMulQuant) return true;      // gemm_launch has checked its layout
+  if (a.epilogue == kEpiSiluMulQuant) return grouped || a.kind == kGemmNvfp4;      // gemm_launch has checked its layout
   if (a.epilogue == kEpiRelu2Quant) return grouped;
   if (a.epilogue != kEpiStore && (grouped || (a.epilogue != kEpiResidual && a.epilogue != kEpiSiluMul))) return false;
   // 16-byte output chunks
@@ -654,7 +685,10 @@ cudaError_t gemm_pair_launch(const GemmArgs& a, cudaStream_t stream) {
   const auto resident_mx = [] {
     int n = resident_clusters<kGemmMxfp4, kEpiStore, false>();
     n = std::min(n, resident_clusters<kGemmMxfp4, kEpiResidual, false>());
-    return std::min(n, resident_clusters<kGemmMxfp4, kEpiSiluMul, false>());
+    n = std::min(n, resident_clusters<kGemmMxfp4, kEpiSiluMul, false>());
+    n = std::min(n, resident_clusters<kGemmMxfp4, kEpiStore, true>());
+    n = std::min(n, resident_clusters<kGemmMxfp4, kEpiRelu2Quant, true>());
+    return std::min(n, resident_clusters<kGemmMxfp4, kEpiSiluMulQuant, true>());
   };
   const bool mx = a.kind == kGemmMxfp4;
   static int known[2][kMaxDevices] = {};      // + 1
@@ -737,7 +771,9 @@ cudaError_t gemm_pair_launch(const GemmArgs& a, cudaStream_t stream) {
 #define HB_PAIR_K(KIND, EPI, GRP) launch<KIND, EPI, GRP>(ta, ta64, ta32, tb, tb_sub, tsfa, tsfb, p, clusters, stream)
 #define HB_PAIR(EPI, GRP) HB_PAIR_K(kGemmNvfp4, EPI, GRP)
   if (mx) switch (a.epilogue) {
-    case kEpiStore: return HB_PAIR_K(kGemmMxfp4, kEpiStore, false);
+    case kEpiStore: return grouped ? HB_PAIR_K(kGemmMxfp4, kEpiStore, true) : HB_PAIR_K(kGemmMxfp4, kEpiStore, false);
+    case kEpiRelu2Quant: return HB_PAIR_K(kGemmMxfp4, kEpiRelu2Quant, true);
+    case kEpiSiluMulQuant: return HB_PAIR_K(kGemmMxfp4, kEpiSiluMulQuant, true);
     case kEpiResidual: return HB_PAIR_K(kGemmMxfp4, kEpiResidual, false);
     case kEpiSiluMul: return HB_PAIR_K(kGemmMxfp4, kEpiSiluMul, false);
     default: return cudaErrorInvalidValue;

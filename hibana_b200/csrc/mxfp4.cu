@@ -116,10 +116,9 @@ quant_mxfp4_kernel(const void* __restrict__ x, long long ldx, int m, int k, int 
     }
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const uint32_t e = top >> 23;                 // 0: zero or below 2^-126, far under the smallest scale
-    const uint32_t b = e == 255u ? 255u : e > 2u ? e - 2u : 0u;
+    float inv;
+    const uint32_t b = mx_scale(top, inv);
     if (c < k) {
-      const float inv = __uint_as_float((b == 255u ? 127u : 254u - b) << 23);
       uint32_t w = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) w |= e2m1x2(f[2 * j] * inv, f[2 * j + 1] * inv) << (8 * j);

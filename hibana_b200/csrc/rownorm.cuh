@@ -21,6 +21,27 @@ __device__ __forceinline__ size_t row_sf_off(int row, int g, int ka) {
   return (static_cast<size_t>(rb) * ka + (g >> 2)) * 512 + (ri & 31) * 16 + (ri >> 5) * 4 + (g & 3);
 }
 
+// Scale byte of a block of 32 in MXFP4 whose largest magnitude has the bits `top` (255: the block holds an infinity or a NaN), and
+// the factor of its numbers.
+__device__ __forceinline__ uint32_t mx_scale(uint32_t top, float& inv) {
+  const uint32_t e = top >> 23;                 // 0: zero or below 2^-126, far under the smallest scale
+  const uint32_t b = e == 255u ? 255u : e > 2u ? e - 2u : 0u;
+  inv = __uint_as_float((b == 255u ? 127u : 254u - b) << 23);
+  return b;
+}
+// Quantises 32 floats to MXFP4: 16 packed bytes and the scale byte.
+__device__ __forceinline__ uint32_t quant32_mx(const float (&x)[32], uint4& packed) {
+  uint32_t top = 0, w[4] = {};
+#pragma unroll
+  for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+  float inv;
+  const uint32_t b = mx_scale(top, inv);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) w[i >> 2] |= e2m1x2(x[2 * i] * inv, x[2 * i + 1] * inv) << (8 * (i & 3));
+  packed = make_uint4(w[0], w[1], w[2], w[3]);
+  return b;
+}
+
 // Quantises 16 floats to NVFP4: writes 8 packed bytes and returns the ue4m3 scale byte (x ~= q * sf * global scale).
 __device__ __forceinline__ uint32_t quant16(const float (&x)[16], float inv_gs, uint2* packed) {
   float amax = 0.f;

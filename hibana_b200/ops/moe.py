@@ -26,7 +26,7 @@ nv.register("hb_moe_plan", [P, I, I, I, I, I, I, P, P, P, P, I, P, I, P, P, I, P
 nv.register("hb_moe_gather", [P, L, P, P, P, I, I, P])
 nv.register("hb_moe_combine", [P, L, P, P, P, L, P, L, I, I, I, P])
 nv.register("hb_gemm_grouped", [I, P, P, P, P, I, I, I, I, P, L, P, I, P, P, I, P, I, I, I, P, P, I, P])
-nv.register("hb_gemm_grouped_quant", [P, P, P, P, I, I, I, I, P, I, P, P, P, I, I, P, P, I, P, P, P, I, L, P])
+nv.register("hb_gemm_grouped_quant", [I, P, P, P, P, I, I, I, I, P, I, P, P, P, I, I, P, P, I, P, P, P, I, L, P])
 nv.register("hb_quant_nvfp4_rows", [P, L, I, I, I, P, P, P, I, P, P, P])
 
 
@@ -300,11 +300,12 @@ def tile_hint(pairs: int, experts: int, max_rows: int, fmt: str) -> int:
 
 
 def pair_rows(ew: "ExpertWeights", max_rows: int) -> bool:
-    """Whether the grouped GEMMs run on SM pairs over 256-row chunks (csrc/gemm_pair.cu): NVFP4 experts as soon as a chunk
+    """Whether the grouped GEMMs run on SM pairs over 256-row chunks (csrc/gemm_pair.cu): FP4 experts as soon as a chunk
     would otherwise be a 128-token tile, in geometries whose activation can be requantised in fc1's epilogue. One-CTA tiles /
     pairs, whole call: 512 experts, top 22, 1024-2688-1024, 129 tokens 603 / 511 us, 256 639 / 531, 904 867 / 560, 4096
-    1910 / 697; 64 experts, top 8, 2048-768-2048 (SwiGLU), 129 tokens 108 / 79, 256 124 / 89, 904 178 / 120, 4096 551 / 236."""
-    return (ew.fmt == "nvfp4" and max_rows > 128 and ew.act in ("swiglu", "relu2") and ew.inter % 64 == 0
+    1910 / 697; 64 experts, top 8, 2048-768-2048 (SwiGLU), 129 tokens 108 / 79, 256 124 / 89, 904 178 / 120, 4096 551 / 236. MXFP4: 664 / 508 and
+    1747 / 668 at 129 and 4096 tokens of the first, 121 / 90 and 535 / 227 of the second."""
+    return (ew.fmt in ("nvfp4", "mxfp4") and max_rows > 128 and ew.act in ("swiglu", "relu2") and ew.inter % 64 == 0
             and ew.n1 % 128 == 0 and ew.fc2_rows % 128 == 0)
 
 
@@ -365,10 +366,18 @@ def experts_forward(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, e
                                      cnt.data_ptr(), max_rows, st.data_ptr(), 0, 0, bn_hint, *tl, nv.stream()), "hb_gemm_grouped")
     elif ew.fmt == "mxfp4":
         q1 = mxfp4.quantize(x, src_rows=src, total_rows=total, rows=rows_cap, gather=True)
-        nv.check(lib.hb_gemm_grouped(4, ew.fc1.q.data_ptr(), q1.q.data_ptr(), ew.fc1.sf.data_ptr(), q1.sf.data_ptr(), e, n1,
-                                     rows_cap, h, h1.data_ptr(), h1.stride(0), None, epi1, start.data_ptr(), cnt.data_ptr(),
-                                     max_rows, st.data_ptr(), ew.fc1.ka, q1.ka, bn_hint, *tl, nv.stream()), "hb_gemm_grouped")
-        q2 = mxfp4.quantize(h1, src_rows=src, total_rows=total)      # (the padding between segments stays as it is)
+        if pairs:
+            q2 = mxfp4.empty(rows_cap, ew.inter, dev)
+            epi = gemm.EPI_SILU_MUL_QUANT if ew.act == "swiglu" else gemm.EPI_RELU2_QUANT
+            nv.check(lib.hb_gemm_grouped_quant(4, ew.fc1.q.data_ptr(), q1.q.data_ptr(), ew.fc1.sf.data_ptr(), q1.sf.data_ptr(), e, n1,
+                                               rows_cap, h, None, epi, start.data_ptr(), cnt.data_ptr(), st.data_ptr(), ew.fc1.ka,
+                                               q1.ka, *tl, q2.q.data_ptr(), q2.sf.data_ptr(), None, q2.ka, ew.inter // 2, nv.stream()),
+                     "hb_gemm_grouped_quant")
+        else:
+            nv.check(lib.hb_gemm_grouped(4, ew.fc1.q.data_ptr(), q1.q.data_ptr(), ew.fc1.sf.data_ptr(), q1.sf.data_ptr(), e, n1,
+                                         rows_cap, h, h1.data_ptr(), h1.stride(0), None, epi1, start.data_ptr(), cnt.data_ptr(),
+                                         max_rows, st.data_ptr(), ew.fc1.ka, q1.ka, bn_hint, *tl, nv.stream()), "hb_gemm_grouped")
+            q2 = mxfp4.quantize(h1, src_rows=src, total_rows=total)      # (the padding between segments stays as it is)
         nv.check(lib.hb_gemm_grouped(4, ew.fc2.q.data_ptr(), q2.q.data_ptr(), ew.fc2.sf.data_ptr(), q2.sf.data_ptr(), e, h_out,
                                      rows_cap, ew.inter, y.data_ptr(), y.stride(0), None, gemm.EPI_STORE, start.data_ptr(),
                                      cnt.data_ptr(), max_rows, st.data_ptr(), ew.fc2.ka, q2.ka, bn_hint, *tl, nv.stream()),
@@ -389,7 +398,7 @@ def experts_forward(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, e
         q2, sf2 = nvfp4._alloc(rows_cap, ew.inter, dev)
         if pairs:
             epi = gemm.EPI_SILU_MUL_QUANT if ew.act == "swiglu" else gemm.EPI_RELU2_QUANT
-            nv.check(lib.hb_gemm_grouped_quant(ew.fc1.q.data_ptr(), q1.data_ptr(), ew.fc1.sf.data_ptr(), sf1.data_ptr(), e, n1,
+            nv.check(lib.hb_gemm_grouped_quant(1, ew.fc1.q.data_ptr(), q1.data_ptr(), ew.fc1.sf.data_ptr(), sf1.data_ptr(), e, n1,
                                                rows_cap, h, ew.fc1_alpha.data_ptr(), epi, start.data_ptr(), cnt.data_ptr(),
                                                st.data_ptr(), ew.fc1.ka, sf1.shape[1], *tl, q2.data_ptr(), sf2.data_ptr(),
                                                ew.fc2_in_scale.data_ptr(), sf2.shape[1], ew.inter // 2, nv.stream()),

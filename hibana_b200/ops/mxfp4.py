@@ -125,6 +125,11 @@ def _alloc(m: int, k: int, device: torch.device) -> tuple[torch.Tensor, torch.Te
             torch.empty(rb, k_atoms(k), 512, dtype=torch.uint8, device=device))
 
 
+def empty(m: int, k: int, device: torch.device) -> Mxfp4Tensor:
+    """An MXFP4 matrix with nothing in it yet."""
+    return Mxfp4Tensor(*_alloc(m, k, device), m, k)
+
+
 def quantize(x: torch.Tensor, *, src_rows: torch.Tensor | None = None, total_rows: torch.Tensor | None = None,
              rows: int | None = None, gather: bool = False) -> Mxfp4Tensor:
     """Rows [M, K] (bf16, fp16 or fp32; any row stride, K a multiple of 32) -> MXFP4.

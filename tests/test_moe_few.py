@@ -300,3 +300,27 @@ def test_a_run_of_them_gpu():
     # what the last projection reads differs by steps of bf16, so some of its codes do
     z2 = gemm.linear_mxfp4(mxfp4.quantize(yg.cpu()), w_out, epilogue=gemm.EPI_RESIDUAL, residual=h)
     assert (zg.cpu().float() - z2.float()).abs().max() <= 2.0 ** -7 * z2.float().abs().max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t,e,k,h,inter,act", [(129, 4, 2, 256, 320, "swiglu"), (300, 6, 3, 288, 384, "relu2"), (520, 8, 2, 128, 128, "relu2"),
+                                               (700, 3, 3, 512, 192, "swiglu"), (129, 40, 1, 96, 128, "swiglu")])
+def test_grouped_mxfp4_experts_on_sm_pairs_gpu(t, e, k, h, inter, act):
+    """Chunks of 256 rows, the activation quantised in the first product's epilogue; a token with an infinity spoils itself only."""
+    ew = _experts(e, h, inter, act, "mxfp4", seed=3, h_out=256)
+    assert moe.pair_rows(ew, t) and not moe.pair_rows(ew, 128)
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn(t, h, generator=g).bfloat16()
+    ids, w = moe.route(torch.randn(t, e, generator=g), k)
+    shared = torch.randn(t, 256, generator=g).bfloat16()
+    ref = moe.experts_forward(x, ids, w, ew, shared=shared).double()
+    ewg = ew.to("cuda")
+    got = moe.experts_forward(x.cuda(), ids.cuda(), w.cuda(), ewg, shared=shared.cuda()).double().cpu()
+    # (as above: codes of mid next to a border may fall on either side)
+    assert (got - ref).norm() <= 2.0 ** -6 * ref.norm()
+    assert torch.equal(moe.experts_forward(x.cuda(), ids.cuda(), w.cuda(), ewg, shared=shared.cuda()).double().cpu(), got)
+    bad = x.clone()
+    bad[t // 2, 5] = float("inf")
+    out = moe.experts_forward(bad.cuda(), ids.cuda(), w.cuda(), ewg, shared=shared.cuda()).double().cpu()
+    keep = torch.arange(t) != t // 2
+    assert torch.equal(out[keep], got[keep]) and out[t // 2].isnan().all() and nv.read_status() == 0
