@@ -211,8 +211,9 @@ def linear_mxfp4(x: Mxfp4Tensor, w: Mxfp4Tensor, *, epilogue: int = EPI_STORE, r
             out.copy_(res)
             return out
         return res
+    given = out is not None
     out = _out(m, n, epilogue, x.q, out)
-    if out.device != x.q.device or out.data_ptr() % 16:
+    if given and (out.device != x.q.device or out.data_ptr() % 16):
         raise ValueError("linear_mxfp4: the output must be on the operands' device and start on a 16-byte boundary")
     if m == 0:
         return out

@@ -109,13 +109,16 @@ def cut(packed: torch.Tensor, scales: torch.Tensor, rows, c0: int, c1: int) -> t
     return packed[rows][:, c0 // 2:c1 // 2], scales[rows][:, c0 // BLOCK:c1 // BLOCK]
 
 
-def _check(x: torch.Tensor) -> None:
-    if x.dim() != 2 or x.dtype not in IN_TYPES:
-        raise ValueError(f"MXFP4: a bf16, fp16 or fp32 matrix expected, got {x.dtype} {tuple(x.shape)}")
-    if x.shape[1] < BLOCK or x.shape[1] % BLOCK:
-        raise ValueError(f"MXFP4: K must be a positive multiple of {BLOCK}, got {x.shape[1]}")
-    if x.shape[0] and x.stride(1) != 1:
+def _check(x: torch.Tensor) -> tuple[int, int]:
+    shape = x.shape
+    if len(shape) != 2 or x.dtype not in IN_TYPES:
+        raise ValueError(f"MXFP4: a bf16, fp16 or fp32 matrix expected, got {x.dtype} {tuple(shape)}")
+    m, k = shape
+    if k < BLOCK or k % BLOCK:
+        raise ValueError(f"MXFP4: K must be a positive multiple of {BLOCK}, got {k}")
+    if m and x.stride(1) != 1:
         raise ValueError("MXFP4: the elements of a row must be contiguous")
+    return m, k
 
 
 def _alloc(m: int, k: int, device: torch.device) -> tuple[torch.Tensor, torch.Tensor]:
@@ -137,12 +140,12 @@ def quantize(x: torch.Tensor, *, src_rows: torch.Tensor | None = None, total_row
     `src_rows` (int32 [rows], CUDA only; the expert-sorted buffers of a mixture-of-experts layer): rows with a negative entry,
     and rows from `total_rows` (int32 [1]) on, are left unwritten; with `gather` output row r is quantised from
     x[src_rows[r]]."""
-    _check(x)
-    m, k = x.shape
-    m = m if rows is None else rows
-    if src_rows is None and (gather or total_rows is not None or m != x.shape[0]):
-        raise ValueError("MXFP4: gather, total_rows and rows go with src_rows")
-    if src_rows is not None:
+    m, k = _check(x)
+    if src_rows is None:
+        if gather or total_rows is not None or (rows is not None and rows != m):
+            raise ValueError("MXFP4: gather, total_rows and rows go with src_rows")
+    else:
+        m = m if rows is None else rows
         if not x.is_cuda or not 0 <= m <= src_rows.numel() or (not gather and m > x.shape[0]):
             raise ValueError(f"MXFP4: {m} rows of {x.shape[0]} by {src_rows.numel()} row numbers on {x.device}")
         for v in (src_rows, total_rows):
@@ -152,7 +155,7 @@ def quantize(x: torch.Tensor, *, src_rows: torch.Tensor | None = None, total_row
         q, sf = _alloc(m, k, x.device)
         if m:
             with nv.on_device(x):
-                nv.check(nv.lib().hb_quant_mxfp4(x.data_ptr(), IN_TYPES[x.dtype], x.stride(0), m, k, sf.shape[1],
+                nv.check(nv.lib().hb_quant_mxfp4(x.data_ptr(), IN_TYPES[x.dtype], x.stride(0), m, k, k_atoms(k),
                                                  q.data_ptr(), sf.data_ptr(), nv.ptr(src_rows), nv.ptr(total_rows),
                                                  int(gather), nv.stream()), "hb_quant_mxfp4")
         return Mxfp4Tensor(q, sf, m, k)
