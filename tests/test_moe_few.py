@@ -324,3 +324,31 @@ def test_grouped_mxfp4_experts_on_sm_pairs_gpu(t, e, k, h, inter, act):
     out = moe.experts_forward(bad.cuda(), ids.cuda(), w.cuda(), ewg, shared=shared.cuda()).double().cpu()
     keep = torch.arange(t) != t // 2
     assert torch.equal(out[keep], got[keep]) and out[t // 2].isnan().all() and nv.read_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4", "bf16"])
+def test_dependent_launches_change_nothing_gpu(fmt):
+    """A chain in which every kernel reads what the one before wrote, with and without programmatic dependent launches."""
+    from hibana_b200.ops import gemm
+    ew, x, rx, router, bias, sh = _case(5, 40, 256, "swiglu", fmt, 128, seed=6)
+    ew, router, sh = ew.to("cuda"), router.cuda(), sh.cuda()
+    g = torch.Generator().manual_seed(7)
+    w = mxfp4.quantize_weight((torch.randn(256, 256, generator=g) * 0.06).cuda())
+
+    def chain():
+        h = x.cuda()
+        for _ in range(12):
+            y = moe.layer_forward(h, router, ew, 4, shared=sh)
+            h = gemm.linear_mxfp4(mxfp4.quantize(y), w, epilogue=gemm.EPI_RESIDUAL, residual=h, static_weight=True)
+            h = h / h.float().abs().amax().clamp_min(1e-6).bfloat16()
+        return h
+
+    gemm.set_pdl(0)
+    try:
+        plain = chain()
+    finally:
+        gemm.set_pdl(2)
+    for _ in range(5):
+        assert torch.equal(chain(), plain)
+    assert not plain.isnan().any() and nv.read_status() == 0
