@@ -21,8 +21,9 @@
 // scale spans 2^-9 .. 2^8; blocks further below the largest of their row share the lowest one. Rows of mid have one scale each, so that
 // half a unit is 2^-14 to 2^-15 of the row's largest number. With bf16 weights x is one column, and mid two (two bf16 numbers, 16 bits).
 //
-// Warp roles (fc1, fc2): one issues the weights' TMA copies into a ring of stages, one the MMAs, two groups of four read accumulators
-// back in turn; in fc2 six convert the rows of mid that a K tile needs, straight into the stage's B tile. fc1 walks (expert, 128
+// Warp roles (fc1, fc2): one issues the weights' TMA copies into a ring of stages; one or two issue MMAs, of two each for every other
+// unit with its own accumulator and its own half of the stages; two groups of four read the accumulators back; in fc2 four convert the rows of
+// mid that a K tile needs, straight into the stage's B tile. fc1 walks (expert, 128
 // rows) over all CTAs with all tokens' columns resident; in fc2 the CTAs of a cluster share an output block of 128 rows, each with its
 // part of the experts, and add up through distributed shared memory in order.
 #include <algorithm>
@@ -43,7 +44,6 @@ constexpr int MAX_PAIRS = MAX_TOKENS * MAX_TOPK;
 constexpr int WARPS = 16;
 constexpr int THREADS = WARPS * 32;
 constexpr int COLS = 8;                  // tokens of an entry of the plan
-constexpr int CONVERTERS = 6;            // warps 2, 3, 12 .. 15
 constexpr int MAX_STAGES = 10;
 constexpr int MAX_CLUSTER = 16;          // of fc2 (more than eight CTAs need a kernel attribute)
 constexpr int MAX_SMEM = 227 * 1024;
@@ -124,19 +124,32 @@ __device__ __forceinline__ uint32_t scale_byte(int e) {
   else return e == 128 ? 0x7Fu : e >= -6 ? static_cast<uint32_t>(e + 7) << 3 : 1u << (e + 9);
 }
 
-// Eight consecutive numbers times f (magnitudes of 2^14 at most) -> five words of eight e2m1 digits.
+// Eight consecutive numbers times f (magnitudes of 2^14 at most; more only in rows that come out as NaN) -> five words of eight e2m1
+// digits. Eighty instructions: with a shift and a table look-up a digit they were 290, and the converters of fc2 were what it waited for.
 __device__ __forceinline__ void digits8(const float (&v)[8], float f, uint32_t (&w)[5]) {
-  // codes of the digits -4 .. 3 (4, which only the top digit takes, has code 6)
-  constexpr uint32_t kCodes = 0x5420ACDEu;
+  // X + 4 + 4 * 8 + .. + 4 * 8^4 is sixteen bits, three a digit (four the top one), rounded by the addition: an fp32 number of this
+  // size counts in ones
+  uint32_t y[4];
 #pragma unroll
-  for (int p = 0; p < 5; ++p) w[p] = 0;
+  for (int j = 0; j < 4; ++j) {
+    constexpr float kOnes = 12582912.f + (4 + 32 + 256 + 2048 + 16384);
+    y[j] = __byte_perm(__float_as_uint(fmaf(v[2 * j], f, kOnes)), __float_as_uint(fmaf(v[2 * j + 1], f, kOnes)), 0x5410);
+  }
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int y = __float2int_rn(fminf(fmaxf(v[j] * f, -16384.f), 16384.f)) + (4 + 32 + 256 + 2048 + 16384);
+  for (int p = 0; p < 5; ++p) {
+    uint32_t sel = 0;                        // digits as indexes: of the even numbers in the lower half, of the odd ones in the upper
 #pragma unroll
-    for (int p = 0; p < 4; ++p) w[p] |= ((kCodes >> (4 * ((y >> (3 * p)) & 7))) & 15u) << (4 * j);
-    const int top_digit = y >> 12;         // 0 .. 8
-    w[4] |= (top_digit == 8 ? 6u : (kCodes >> (4 * top_digit)) & 15u) << (4 * j);
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t at = 4 * j >= 3 * p ? y[j] << (4 * j - 3 * p) : y[j] >> (3 * p - 4 * j);
+      sel |= at & ((p == 4 ? 0x000F000Fu : 0x00070007u) << (4 * j));
+    }
+    // codes of the digits -4 .. 3, a byte each; 4, which only the top digit takes, is the code of -4 without its sign
+    uint32_t even = __byte_perm(0x0A0C0D0Eu, 0x05040200u, sel & 0x7777u), odd = __byte_perm(0x0A0C0D0Eu, 0x05040200u, (sel >> 16) & 0x7777u);
+    if (p == 4) {
+      even ^= __byte_perm(0u, 8u, (sel >> 1) & 0x4444u);
+      odd ^= __byte_perm(0u, 8u, (sel >> 17) & 0x4444u);
+    }
+    w[p] = even | odd << 4;
   }
 }
 // A block whose largest magnitude (bits) is `top`: the factor of its numbers, 2^(140 - e) with e the biased exponent of `top`, and the
@@ -478,12 +491,15 @@ __host__ __device__ inline int fc1_fixed_bytes(int tokens, int n, int hidden) {
   return 1024 + k_tiles_of(hidden, T::TILE_K) * (n * 128 + T::SF_BYTES) + tokens * CAND_BYTES + align_to(sizeof(Plan), 16) + BAR_BYTES;
 }
 template <int KIND>
-__host__ __device__ inline int fc2_fixed_bytes(int tokens) {
+__host__ __device__ constexpr int fc2_fixed_bytes(int tokens) {
   return 1024 + 2 * tokens * 512 + 512 + align_to(sizeof(Plan), 16) + BAR_BYTES;
 }
-constexpr int ACC_COLS = 96;              // two accumulators, then scales of A (a tile's) and of B (all tiles' where they fit)
-constexpr int SFA_COL = 192, SFB_COL = 208;
+constexpr int ACC_COLS = 96;              // two accumulators, then scales of A (a tile's of each) and of B (all tiles' where they fit)
+constexpr int SFA_COL = 192, SFB_COL = 224;
 constexpr int TMEM_COLS = 512;
+// Warps that issue MMAs, each with its share of the stages.
+template <int KIND, bool SECOND>
+constexpr int streams() { return SECOND || KIND == kGemmBf16 ? 2 : 1; }
 
 template <int KIND, bool SECOND>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -491,6 +507,7 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
   using T = Traits<KIND>;
   constexpr int STAGE = SECOND ? T::STAGE2 : T::STAGE1;
   constexpr int P = SECOND ? T::MP : T::XP;
+  constexpr int STREAMS = streams<KIND, SECOND>();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -508,7 +525,8 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
   uint64_t* accum = b_full + MAX_STAGES;      // [2] accumulator complete
   uint64_t* acc_free = accum + 2;             // [2] and read back (four warps)
   uint64_t* x_full = acc_free + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(x_full + 1);
+  uint64_t* sfb_full = x_full + 1;            // scales of B that stay are in tensor memory
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sfb_full + 1);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
   uint32_t cluster_n = 1, cluster_rank = 0;
   if constexpr (SECOND) {
@@ -527,6 +545,7 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
       mbar_init(&acc_free[i], 4);
     }
     mbar_init(x_full, 1);
+    mbar_init(sfb_full, 1);
     *abort = 0;
     fence_mbar_init();
     prefetch_tmap(&tw);
@@ -630,29 +649,48 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
     __syncthreads();
   }
 
+  // With two streams units go in pairs, K tile by K tile: the first's stages are the even ones, the second's the odd ones (S is even).
+  // (A K tile's waits, copies of scales, MMAs and commits take one warp 460 cycles: 16 KB a 0.24 us, where 120 SMs' share of the memory's
+  // rate is 0.31. fc2 of 7 tokens over 64 bf16 experts: 38 us with one, 31 with two; its fc1 53, 49. The FP4 fc1, with memory's rate and
+  // with few stages beside 16 rows of x, lost 4 us of 51.)
   const uint32_t ring_addr = __shfl_sync(0xffffffffu, smem_u32(ring), 0), xsf_addr = __shfl_sync(0xffffffffu, smem_u32(xsf), 0);
   if (warp == 0) {
     // ---- weights: the whole warp walks the loop (waits included), one elected lane issues
-    int i = 0, s = 0;
+    int i = 0, s = 0, alone = 0x7FFFFFFF;      // place in the ring's order; from `alone` on every other one is left out
     uint32_t phase = 1;                       // (the first round finds every stage free)
     bool ok = true;
-    for (int u = u0; u < units && ok; u += stride) {
-      const int entry = u / tiles;
-      const int row0 = __shfl_sync(0xffffffffu, static_cast<int>(plan.expert[entry]) * rows_per_expert +
-                                                    (SECOND ? out_block : u - entry * tiles) * 128, 0);
-      for (int kt = 0; kt < k_tiles; ++kt, ++i) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], phase, abort, p.status, kTimeoutEmpty));
-        if (!ok) break;
-        if (elect_one()) {
-          const uint32_t st = ring_addr + s * STAGE, bar = smem_u32(&full[s]);
-          mbar_expect_tx(&full[s], A_BYTES + T::SF_BYTES);
-          tma_load_2d_once(st, &tw, bar, kt * (T::kFp4 ? 128 : 64), row0);
-          if constexpr (T::kFp4)
-            bulk_load(st + A_BYTES, (SECOND ? p.sf2 : p.sf1) + (static_cast<size_t>(row0 >> 7) * (SECOND ? p.ka2 : p.ka1) + kt * T::ATOMS) * 512,
-                      T::SF_BYTES, bar);
+    for (int u = u0; u < units && ok; u += STREAMS * stride) {
+      const int of_pair = STREAMS == 2 && u + stride < units ? 2 : 1;
+      if (STREAMS == 2 && of_pair == 1) alone = i;
+      int rows[STREAMS];
+#pragma unroll
+      for (int h = 0; h < STREAMS; ++h) {
+        const int v = h < of_pair ? u + h * stride : u, entry = v / tiles;
+        rows[h] = __shfl_sync(0xffffffffu, static_cast<int>(plan.expert[entry]) * rows_per_expert +
+                                               (SECOND ? out_block : v - entry * tiles) * 128, 0);
+      }
+      for (int kt = 0; kt < k_tiles && ok; ++kt) {
+#pragma unroll
+        for (int h = 0; h < STREAMS; ++h) {
+          if (h >= of_pair || !ok) break;
+          const int at = s + h, row0 = rows[h];
+          ok = __all_sync(0xffffffffu, mbar_wait(&empty[at], phase, abort, p.status, kTimeoutEmpty));
+          if (!ok) break;
+          if (elect_one()) {
+            const uint32_t st = ring_addr + at * STAGE, bar = smem_u32(&full[at]);
+            mbar_expect_tx(&full[at], A_BYTES + T::SF_BYTES);
+            tma_load_2d_once(st, &tw, bar, kt * (T::kFp4 ? 128 : 64), row0);
+            if constexpr (T::kFp4)
+              bulk_load(st + A_BYTES, (SECOND ? p.sf2 : p.sf1) + (static_cast<size_t>(row0 >> 7) * (SECOND ? p.ka2 : p.ka1) + kt * T::ATOMS) * 512,
+                        T::SF_BYTES, bar);
+          }
+          __syncwarp();
+          ++i;
         }
-        __syncwarp();
-        if (++s == S) {
+        if (!ok) break;
+        i += STREAMS - of_pair;
+        s += STREAMS;
+        if (s == S) {
           s = 0;
           phase ^= 1;
         }
@@ -660,12 +698,14 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
     }
     if (!ok && lane == 0) {                   // bounded wait for the copies still in flight: none may land after the CTA has gone
       volatile int ignore = 0;
-      for (int j = max(i - S, 0); j < i; ++j) mbar_wait(&full[j % S], (j / S) & 1, &ignore, nullptr, kTimeoutDrain);
+      for (int j = max(i - S, 0); j < i; ++j)
+        if (j < alone || (j & 1) == 0) mbar_wait(&full[j % S], (j / S) & 1, &ignore, nullptr, kTimeoutDrain);
     }
     __syncwarp();
-  } else if (warp == 1) {
+  } else if (warp == 1 || (STREAMS == 2 && warp == 3)) {
     // ---- products
-    int s = 0, it = 0;
+    const int set = warp >> 1;
+    int s = set, it = 0;                      // (of this warp's units)
     uint32_t phase = 0;
     bool ok = true, ready = false;
     if constexpr (!SECOND) ok = __all_sync(0xffffffffu, mbar_wait(x_full, 0, abort, p.status, kTimeoutFull));
@@ -674,15 +714,20 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
     const bool resident = SECOND || SFB_COL + k_tiles * T::ATOMS * 4 <= TMEM_COLS;
     if constexpr (T::kFp4) {
       tc_fence_after();
-      if (resident && ok && elect_one())
+      if (resident && set == 0 && ok && elect_one()) {
         for (int at = 0; at < (SECOND ? 1 : k_tiles * T::ATOMS); ++at)
           tmem_cp_32x128b_x4(tmem + SFB_COL + at * 4, make_desc_sf(xsf_addr + at * 512));
+        tc_commit(sfb_full);
+      }
       __syncwarp();
+      if (resident && set == 1 && u0 + stride < units && ok) ok = __all_sync(0xffffffffu, mbar_wait(sfb_full, 0, abort, p.status, kTimeoutAccum));
     }
-    for (int u = u0; u < units && ok; u += stride, ++it) {
+    const uint32_t sfa = tmem + SFA_COL + set * 16;
+    for (int u = u0 + set * stride; u < units && ok; u += STREAMS * stride, ++it) {
+      const int buf = STREAMS == 2 ? set : it & 1, turn = STREAMS == 2 ? it : it >> 1;      // accumulator, and its how manieth use
+      const uint32_t acc = tmem + buf * ACC_COLS;
       const int n = __shfl_sync(0xffffffffu, SECOND ? (plan.count[u] * P + 15) / 16 * 16 : p.n, 0);
-      const uint32_t acc = tmem + (it & 1) * ACC_COLS;
-      if (it >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&acc_free[it & 1], ((it >> 1) - 1) & 1, abort, p.status, kTimeoutAccum));
+      if (turn >= 1) ok = __all_sync(0xffffffffu, mbar_wait(&acc_free[buf], (turn - 1) & 1, abort, p.status, kTimeoutAccum));
       if (!ok) break;
       tc_fence_after();
       for (int kt = 0; kt < k_tiles; ++kt) {
@@ -693,21 +738,23 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
         if (!ok) break;
         tc_fence_after();
         const int s_at = s;
-        if (++s == S) {
-          s = 0;
+        s += STREAMS;
+        if (s >= S) {
+          s = set;
           phase ^= 1;
         }
-        // of the next tile, answered while this one is issued: a wait that finds its barrier complete takes 0.1 us all the same
-        const bool peek = mbar_test_wait(&full[s], phase) && (!SECOND || mbar_test_wait(&b_full[s], phase));
+        // Of the next tile, answered while this one is issued: a wait that finds its barrier complete takes 0.1 us all the same. In fc2
+        // odd lanes ask for B: one test of both.
+        const bool peek = mbar_test_wait((SECOND && (lane & 1) ? b_full : full) + s, phase);
         const uint32_t st = ring_addr + s_at * STAGE;
         const uint32_t b_at = SECOND ? st + A_BYTES + T::SF_BYTES : ring_addr - x_bytes + kt * p.n * 128;
-        const uint32_t sfb = tmem + SFB_COL + (!SECOND && resident ? kt * T::ATOMS * 4 : 0);
+        const uint32_t sfb = tmem + SFB_COL + (SECOND ? 0 : resident ? kt * T::ATOMS * 4 : set * 16);
         const uint64_t adesc = make_desc_sw128(st), bdesc = make_desc_sw128(b_at);
         const int mmas = min(4, (K - kt * T::TILE_K + T::MMA_K - 1) / T::MMA_K);
         if (elect_one()) {
           if constexpr (T::kFp4) {
 #pragma unroll
-            for (int at = 0; at < T::ATOMS; ++at) tmem_cp_32x128b_x4(tmem + SFA_COL + at * 4, make_desc_sf(st + A_BYTES + at * 512));
+            for (int at = 0; at < T::ATOMS; ++at) tmem_cp_32x128b_x4(sfa + at * 4, make_desc_sf(st + A_BYTES + at * 512));
             if (!SECOND && !resident) {
 #pragma unroll
               for (int at = 0; at < T::ATOMS; ++at) tmem_cp_32x128b_x4(sfb + at * 4, make_desc_sf(xsf_addr + kt * T::SF_BYTES + at * 512));
@@ -719,15 +766,15 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
             const uint32_t more = kt > 0 || kb > 0 ? 1u : 0u;
             if constexpr (KIND == kGemmMxfp4)
               mma_mxf4(acc, adesc + kb * 2, bdesc + kb * 2, make_idesc_mxf4(128, 0, kb & 1) | static_cast<uint32_t>(n >> 3) << 17, more,
-                       tmem + SFA_COL + (kb >> 1) * 4, SECOND ? sfb : sfb + (kb >> 1) * 4);
+                       sfa + (kb >> 1) * 4, SECOND ? sfb : sfb + (kb >> 1) * 4);
             else if constexpr (KIND == kGemmNvfp4)
               mma_nvf4(acc, adesc + kb * 2, bdesc + kb * 2, make_idesc_nvf4(128, 0) | static_cast<uint32_t>(n >> 3) << 17, more,
-                       tmem + SFA_COL + kb * 4, SECOND ? sfb : sfb + kb * 4);
+                       sfa + kb * 4, SECOND ? sfb : sfb + kb * 4);
             else
               mma_f16(acc, adesc + kb * 2, bdesc + kb * 2, make_idesc_bf16(128, 0) | static_cast<uint32_t>(n >> 3) << 17, more);
           }
           tc_commit(&empty[s_at]);
-          if (kt == k_tiles - 1) tc_commit(&accum[it & 1]);
+          if (kt == k_tiles - 1) tc_commit(&accum[buf]);
         }
         ready = __all_sync(0xffffffffu, peek);
       }
@@ -778,51 +825,54 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
         }
       }
     }
-  } else if (SECOND) {
-    // ---- rows of mid: converter j writes the B tile of every CONVERTERS-th K tile
-    const int j = warp < 4 ? warp - 2 : warp - 10;
-    int next = j, s = 0;                      // tiles until this warp's next one; the stage of the tile at hand
+  } else if (SECOND && warp >= 12) {
+    // ---- rows of mid: two warps write the B tiles of the even stages in turn, two those of the odd ones. (A warp sees two of a stage's
+    // uses apart by its parity only, so the tiles it takes are never more than a ring apart among those of one MMA warp.)
+    const int set = warp & 1;
+    int s = set, turns = (warp >> 1) & 1;     // the stage of the tile at hand; tiles until this warp's next one
     uint32_t phase = 1;
     bool ok = true;
-    for (int u = u0; u < units && ok; u += stride) {
+    for (int u = u0 + set * stride; u < units && ok; u += 2 * stride) {
       const int n = plan.count[u];
       for (int kt = 0; kt < k_tiles; ++kt) {
         const int mine = s;
         const uint32_t turn = phase;
-        if (++s == S) {
-          s = 0;
+        s += 2;
+        if (s >= S) {
+          s = set;
           phase ^= 1;
         }
-        if (next-- != 0) continue;
-        next = CONVERTERS - 1;
+        if (turns-- != 0) continue;
+        turns = 1;
+        // (of FP4 a warp takes a row at a time, of bf16 four; the first numbers are under way before the stage is free)
+        constexpr int LANES = T::TILE_K / 8, STEP = 32 / LANES;
+        const int k = kt * T::TILE_K + (lane % LANES) * 8;
+        float v[8], next[8];
+        auto fetch = [&](int c, float (&to)[8]) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) to[e] = 0.f;
+          if (c < n && k < p.inter) {
+            const float4* at = reinterpret_cast<const float4*>(p.mid + static_cast<size_t>(plan.pair[u * COLS + c]) * p.inter + k);
+            const float4 lo = ld_step(at), hi = ld_step(at + 1);
+            to[0] = lo.x; to[1] = lo.y; to[2] = lo.z; to[3] = lo.w; to[4] = hi.x; to[5] = hi.y; to[6] = hi.z; to[7] = hi.w;
+          }
+        };
+        fetch(lane / LANES, next);
         ok = __all_sync(0xffffffffu, mbar_wait(&empty[mine], turn, abort, p.status, kTimeoutEmpty));
         if (!ok) break;
         uint8_t* b = ring + mine * STAGE + A_BYTES + T::SF_BYTES;
-        if constexpr (T::kFp4) {
-          const int k = kt * T::TILE_K + lane * 8;
-#pragma unroll 2
-          for (int c = 0; c < n; ++c) {
-            const int pr = plan.pair[u * COLS + c];
-            const float* row = p.mid + static_cast<size_t>(pr) * p.inter;
-            float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (k < p.inter) {
-              const float4 lo = ld_step(reinterpret_cast<const float4*>(row + k)), hi = ld_step(reinterpret_cast<const float4*>(row + k + 4));
-              v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w; v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
-            }
+#pragma unroll 1
+        for (int c = lane / LANES; c < n; c += STEP) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = next[e];
+          fetch(c + STEP, next);
+          if constexpr (T::kFp4) {
             uint32_t w[5];
-            digits8(v, mid_factor(plan.row_exp[pr]), w);
+            digits8(v, mid_factor(plan.row_exp[plan.pair[u * COLS + c]]), w);
 #pragma unroll
             for (int d = 0; d < 5; ++d) *reinterpret_cast<uint32_t*>(b + b_offset(c * 5 + d, lane * 4)) = w[d];
-          }
-        } else {
-          for (int c = lane >> 3; c < n; c += 4) {
-            const float* row = p.mid + static_cast<size_t>(plan.pair[u * COLS + c]) * p.inter;
-            const int k = kt * T::TILE_K + (lane & 7) * 8;
-            float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, h[8];
-            if (k < p.inter) {
-              const float4 lo = ld_step(reinterpret_cast<const float4*>(row + k)), hi = ld_step(reinterpret_cast<const float4*>(row + k + 4));
-              v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w; v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
-            }
+          } else {
+            float h[8];
             const uint4 top = pack8(v);
             unpack8(top, h);
 #pragma unroll
@@ -901,7 +951,8 @@ int resident(int size) {
 
 template <int KIND>
 int fc1_stages(int tokens, int n, int hidden) {
-  return std::min(MAX_STAGES, (MAX_SMEM - fc1_fixed_bytes<KIND>(tokens, n, hidden)) / Traits<KIND>::STAGE1);
+  const int s = std::min(MAX_STAGES, (MAX_SMEM - fc1_fixed_bytes<KIND>(tokens, n, hidden)) / Traits<KIND>::STAGE1);
+  return streams<KIND, false>() == 2 ? s & ~1 : s;
 }
 int columns(int tokens, int per) { return (tokens * per + 15) / 16 * 16; }
 
@@ -969,7 +1020,8 @@ cudaError_t launch_few(FewParams& p, const void* w1, const void* w2, uint8_t* ws
   p.stages = fc1_stages<KIND>(p.tokens, p.n, p.hidden);
   e = launch_dep(k1, dim3(kNumSms), dim3(THREADS), MAX_SMEM, st, t1, p);
   if (e != cudaSuccess) return e;
-  p.stages = std::min(MAX_STAGES, (MAX_SMEM - fc2_fixed_bytes<KIND>(p.tokens)) / T::STAGE2);
+  static_assert((MAX_SMEM - fc2_fixed_bytes<KIND>(MAX_TOKENS)) / T::STAGE2 >= 4, "what the converters' waits rest on");
+  p.stages = std::min(MAX_STAGES, (MAX_SMEM - fc2_fixed_bytes<KIND>(p.tokens)) / T::STAGE2) & ~1;
   // CTAs of a cluster share an output block's experts: the number that leaves each the least to do
   const int blocks = (p.h_out + 127) / 128;
   int cluster = 1;
