@@ -6,6 +6,7 @@
 //   mid_j  = silu(W1g x) * (W1u x)  or  relu(W1 x)^2          W1, W2 of expert ids_j
 //   out    = sum_j w_j W2 mid_j (+ shared)                    rounded once
 //
+// Three launches:
 //   route : router logits; the rows of x as an operand of the tensor cores;
 //   fc1   : top-k and plan, the chosen experts' first product, the activation;
 //   fc2   : the second product, the weighted sum, the shared expert's rows.
@@ -21,11 +22,19 @@
 // scale spans 2^-9 .. 2^8; blocks further below the largest of their row share the lowest one. Rows of mid have one scale each, so that
 // half a unit is 2^-14 to 2^-15 of the row's largest number. With bf16 weights x is one column, and mid two (two bf16 numbers, 16 bits).
 //
-// Warp roles (fc1, fc2): one issues the weights' TMA copies into a ring of stages; one or two issue MMAs, of two each for every other
-// unit with its own accumulator and its own half of the stages; two groups of four read the accumulators back; in fc2 four convert the rows of
+// Warp roles (fc1, fc2): one issues the weights' TMA copies into a ring of stages; one or two (each for every other unit, with its own
+// accumulator and its own half of the stages) issue MMAs; two groups of four read the accumulators back; in fc2 four convert the rows of
 // mid that a K tile needs, straight into the stage's B tile. fc1 walks (expert, 128
 // rows) over all CTAs with all tokens' columns resident; in fc2 the CTAs of a cluster share an output block of 128 rows, each with its
 // part of the experts, and add up through distributed shared memory in order.
+//
+// Measured (us a call among others, weights from memory; in brackets route / fc1 / fc2 on their own, and the time of the bytes at the copy
+// rate): 512 experts, 2560-640 SwiGLU, MXFP4, top 10: 1 token 25 (4.0 / 14 / 15.5; 4.4), 16 tokens 78 (4.4 / 50 / 36; 56); 512
+// experts, 1024-2688 squared ReLU, NVFP4, top 22, router over 4096: 4 tokens 60 (5.8 / 33 / 34; 40); 64 experts, 2048-768 SwiGLU, bf16,
+// top 8: 7 tokens 69 (3.5 / 48 / 31; 56). The products stream 5 to 6.6 TB/s while they stream. Bound by what happens before the first
+// weights can be named and between kernels: logits 4, top-k and plan 4, first tiles 2 each, from fc1's last tile to fc2's first 5, the
+// cluster's sums 3. fc2 runs on the clusters that fit (80 to 120 of 148 SMs: 120 with clusters of six on 20 output blocks). Fetching the
+// first of W2 into L2 from fc1's last tiles on made 16 tokens 2 us slower.
 #include <algorithm>
 #include <cstddef>
 
@@ -497,9 +506,6 @@ __host__ __device__ constexpr int fc2_fixed_bytes(int tokens) {
 constexpr int ACC_COLS = 96;              // two accumulators, then scales of A (a tile's of each) and of B (all tiles' where they fit)
 constexpr int SFA_COL = 192, SFB_COL = 224;
 constexpr int TMEM_COLS = 512;
-// Warps that issue MMAs, each with its share of the stages.
-template <int KIND, bool SECOND>
-constexpr int streams() { return SECOND || KIND == kGemmBf16 ? 2 : 1; }
 
 template <int KIND, bool SECOND>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -507,14 +513,13 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
   using T = Traits<KIND>;
   constexpr int STAGE = SECOND ? T::STAGE2 : T::STAGE1;
   constexpr int P = SECOND ? T::MP : T::XP;
-  constexpr int STREAMS = streams<KIND, SECOND>();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-  const int S = p.stages, K = SECOND ? p.inter : p.hidden, k_tiles = k_tiles_of(K, T::TILE_K);
+  const int K = SECOND ? p.inter : p.hidden, k_tiles = k_tiles_of(K, T::TILE_K);
   const int x_bytes = SECOND ? 0 : k_tiles * p.n * 128, xsf_bytes = SECOND ? 0 : k_tiles * T::SF_BYTES;
   uint8_t* ring = sm + x_bytes;
-  uint8_t* after = ring + S * STAGE;
+  uint8_t* after = ring + p.stages * STAGE;
   float* sums = reinterpret_cast<float*>(after);                                // fc2: [2][tokens][128]
   uint8_t* xsf = SECOND ? after + 2 * p.tokens * 512 : after;                   // scales of operand B
   uint8_t* plan_at = after + (SECOND ? 2 * p.tokens * 512 + 512 : xsf_bytes + p.tokens * CAND_BYTES);
@@ -649,29 +654,36 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
     __syncthreads();
   }
 
-  // With two streams units go in pairs, K tile by K tile: the first's stages are the even ones, the second's the odd ones (S is even).
-  // (A K tile's waits, copies of scales, MMAs and commits take one warp 460 cycles: 16 KB a 0.24 us, where 120 SMs' share of the memory's
-  // rate is 0.31. fc2 of 7 tokens over 64 bf16 experts: 38 us with one, 31 with two; its fc1 53, 49. The FP4 fc1, with memory's rate and
-  // with few stages beside 16 rows of x, lost 4 us of 51.)
+  // Streams: warps that issue MMAs, each with its share of the stages. A K tile's waits, copies of scales, MMAs and commits take one warp
+  // 460 cycles, 0.24 us; the 16 KB of one on each of 120 SMs are 0.3 at memory's rate, on fewer SMs less. fc2 with one warp and with two,
+  // 8 and 16 tokens: 256 bf16 experts, top 22, 1024-2688 169 / 149 and 238 / 213 us, 512 MXFP4 ones 63 / 57 and 100 / 85; 256 of bf16,
+  // top 10, 2560-640 56 / 54 and 83 / 82. fc1 has all SMs, and a unit without a second has half the stages, so two streams lose where
+  // every CTA has work to the end (16 tokens over 64 bf16 experts 67 / 70, 512 MXFP4 ones 51 / 55) or the last units stand alone (one
+  // token 21 / 25). They win where the last round is the second of a pair and sparse: the CTAs with one unit more then have it beside
+  // their last but one (8 tokens over 64 bf16 experts 54 / 51, one over 256, top 22, 33 / 29).
+  const int rounds = (units + stride - 1) / stride;
+  const bool two = SECOND || (p.stages >= 6 && rounds % 2 == 0 && 2 * (rounds * stride - units) >= stride);
+  const int streams = two ? 2 : 1, S = two ? p.stages & ~1 : p.stages;
+  // With two streams units go in pairs, K tile by K tile: the first's stages are the even ones, the second's the odd ones.
   const uint32_t ring_addr = __shfl_sync(0xffffffffu, smem_u32(ring), 0), xsf_addr = __shfl_sync(0xffffffffu, smem_u32(xsf), 0);
   if (warp == 0) {
     // ---- weights: the whole warp walks the loop (waits included), one elected lane issues
     int i = 0, s = 0, alone = 0x7FFFFFFF;      // place in the ring's order; from `alone` on every other one is left out
     uint32_t phase = 1;                       // (the first round finds every stage free)
     bool ok = true;
-    for (int u = u0; u < units && ok; u += STREAMS * stride) {
-      const int of_pair = STREAMS == 2 && u + stride < units ? 2 : 1;
-      if (STREAMS == 2 && of_pair == 1) alone = i;
-      int rows[STREAMS];
+    for (int u = u0; u < units && ok; u += streams * stride) {
+      const int of_pair = two && u + stride < units ? 2 : 1;
+      if (two && of_pair == 1) alone = i;
+      int rows[2];
 #pragma unroll
-      for (int h = 0; h < STREAMS; ++h) {
+      for (int h = 0; h < 2; ++h) {
         const int v = h < of_pair ? u + h * stride : u, entry = v / tiles;
         rows[h] = __shfl_sync(0xffffffffu, static_cast<int>(plan.expert[entry]) * rows_per_expert +
                                                (SECOND ? out_block : v - entry * tiles) * 128, 0);
       }
       for (int kt = 0; kt < k_tiles && ok; ++kt) {
 #pragma unroll
-        for (int h = 0; h < STREAMS; ++h) {
+        for (int h = 0; h < 2; ++h) {
           if (h >= of_pair || !ok) break;
           const int at = s + h, row0 = rows[h];
           ok = __all_sync(0xffffffffu, mbar_wait(&empty[at], phase, abort, p.status, kTimeoutEmpty));
@@ -688,8 +700,8 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
           ++i;
         }
         if (!ok) break;
-        i += STREAMS - of_pair;
-        s += STREAMS;
+        i += streams - of_pair;
+        s += streams;
         if (s == S) {
           s = 0;
           phase ^= 1;
@@ -702,7 +714,7 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
         if (j < alone || (j & 1) == 0) mbar_wait(&full[j % S], (j / S) & 1, &ignore, nullptr, kTimeoutDrain);
     }
     __syncwarp();
-  } else if (warp == 1 || (STREAMS == 2 && warp == 3)) {
+  } else if (warp == 1 || (two && warp == 3)) {
     // ---- products
     const int set = warp >> 1;
     int s = set, it = 0;                      // (of this warp's units)
@@ -723,8 +735,8 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
       if (resident && set == 1 && u0 + stride < units && ok) ok = __all_sync(0xffffffffu, mbar_wait(sfb_full, 0, abort, p.status, kTimeoutAccum));
     }
     const uint32_t sfa = tmem + SFA_COL + set * 16;
-    for (int u = u0 + set * stride; u < units && ok; u += STREAMS * stride, ++it) {
-      const int buf = STREAMS == 2 ? set : it & 1, turn = STREAMS == 2 ? it : it >> 1;      // accumulator, and its how manieth use
+    for (int u = u0 + set * stride; u < units && ok; u += streams * stride, ++it) {
+      const int buf = two ? set : it & 1, turn = two ? it : it >> 1;      // accumulator, and its use
       const uint32_t acc = tmem + buf * ACC_COLS;
       const int n = __shfl_sync(0xffffffffu, SECOND ? (plan.count[u] * P + 15) / 16 * 16 : p.n, 0);
       if (turn >= 1) ok = __all_sync(0xffffffffu, mbar_wait(&acc_free[buf], (turn - 1) & 1, abort, p.status, kTimeoutAccum));
@@ -738,7 +750,7 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
         if (!ok) break;
         tc_fence_after();
         const int s_at = s;
-        s += STREAMS;
+        s += streams;
         if (s >= S) {
           s = set;
           phase ^= 1;
@@ -951,8 +963,7 @@ int resident(int size) {
 
 template <int KIND>
 int fc1_stages(int tokens, int n, int hidden) {
-  const int s = std::min(MAX_STAGES, (MAX_SMEM - fc1_fixed_bytes<KIND>(tokens, n, hidden)) / Traits<KIND>::STAGE1);
-  return streams<KIND, false>() == 2 ? s & ~1 : s;
+  return std::min(MAX_STAGES, (MAX_SMEM - fc1_fixed_bytes<KIND>(tokens, n, hidden)) / Traits<KIND>::STAGE1);
 }
 int columns(int tokens, int per) { return (tokens * per + 15) / 16 * 16; }
 

@@ -428,7 +428,9 @@ def experts_forward(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, e
     return out
 
 
-FEW_TOKENS = 16          # tokens up to which a layer runs in csrc/moe_few.cu
+# Tokens up to which a layer runs in csrc/moe_few.cu. Whole layers in graphs, weights from memory, few-token / grouped form: 512 experts,
+# top 10, 2560-640, shared expert, 16 tokens: NVFP4 121 / 158 us, MXFP4 117 / 172; 512 experts, top 22, 1024-2688: 229 / 258, 207 / 291.
+FEW_TOKENS = 16
 _KINDS = {"bf16": 0, "nvfp4": 1, "mxfp4": 4}
 
 nv.register("hb_moe_few_tokens", [I, I])
@@ -475,8 +477,8 @@ def layer_forward(x: torch.Tensor, router: torch.Tensor, ew: ExpertWeights, topk
     """A whole mixture-of-experts layer: x [T, H] bf16 -> [T, H_out] bf16.
 
     router bf16 [E, Hr]; its input rows are `route_x` [T, Hr] (a latent layer routes on the hidden rows) or x. Scores, top-k and
-    weights as in `route`; `shared` [T, H_out] bf16 is added to the sum. Up to FEW_TOKENS tokens the layer is two kernels
-    that stream the chosen experts' weights once and read the activations in bf16, whatever the experts' format; more
+    weights as in `route`; `shared` [T, H_out] bf16 is added to the sum. Up to FEW_TOKENS tokens the layer is three kernels
+    (logits; both products) that stream the chosen experts' weights once and read the activations in bf16, whatever the experts' format; more
     tokens, and layers `few_tokens_ok` does not cover, take `linear_bf16`, `route` and `experts_forward` (which quantises
     activations for FP4 experts)."""
     if x.dim() != 2 or x.dtype != torch.bfloat16 or x.shape[1] != ew.hidden:

@@ -1,4 +1,4 @@
-"""A mixture-of-experts layer for a few tokens (two kernels) against a plain computation in 64 bits; MXFP4 experts."""
+"""A mixture-of-experts layer for a few tokens against a plain computation in 64 bits; MXFP4 experts."""
 import pytest
 import torch
 
