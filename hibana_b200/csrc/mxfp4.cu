@@ -82,24 +82,25 @@ struct Raw8 {
   }
 };
 
-// src_rows (may be null; the expert-sorted buffers of a mixture-of-experts layer): rows with a negative entry are padding and
-// are left alone; with `gather` output row r takes input row src_rows[r]. Rows from *total_rows on are left alone too.
+// dst_rows (may be null; the expert-sorted buffers of a mixture-of-experts layer, m pairs of a token and one of its topk experts): pair r
+// goes to row dst_rows[r], of token r / topk or, with topk 0, of the same row of x; a negative entry leaves the pair out. The other rows
+// of the buffers (most of them, with few tokens: every expert's segment is padded to 128) are not touched.
 template <int IN, bool VEC>
 __global__ void __launch_bounds__(QUANT_WARPS * 32, IN == kInF32 ? 9 : 16)
 quant_mxfp4_kernel(const void* __restrict__ x, long long ldx, int m, int k, int ka, uint8_t* __restrict__ q,
-                   uint8_t* __restrict__ sf, int segs, const int* __restrict__ src_rows, const int* __restrict__ total_rows,
-                   int gather) {
-  grid_dep_wait(x, src_rows, total_rows);
+                   uint8_t* __restrict__ sf, int segs, const int* __restrict__ dst_rows, int topk) {
+  grid_dep_wait(x, dst_rows);
   grid_dep_launch();      // behind the wait: a grouped GEMM that follows reads the routing plan at once (see launch_dep)
   const uint32_t unit = blockIdx.x * QUANT_WARPS + (threadIdx.x >> 5);      // (the launch keeps it below 2^31)
   const int row = static_cast<int>(unit / static_cast<uint32_t>(segs)), seg = static_cast<int>(unit) - row * segs;
   const int lane = threadIdx.x & 31;
-  if (row >= m || (total_rows != nullptr && row >= *total_rows)) return;
+  if (row >= m) return;
   long long in_row = row;
-  if (src_rows != nullptr) {
-    const int s = src_rows[row];
-    if (s < 0) return;
-    if (gather) in_row = s;
+  int dst = row;
+  if (dst_rows != nullptr) {
+    dst = dst_rows[row];
+    if (dst < 0) return;
+    in_row = topk > 0 ? row / topk : dst;
   }
   const long long base = in_row * ldx;
   const int k0 = seg * SEG + lane * 8;
@@ -125,14 +126,14 @@ quant_mxfp4_kernel(const void* __restrict__ x, long long ldx, int m, int k, int 
       uint32_t w = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) w |= e2m1x2(f[2 * j] * inv, f[2 * j + 1] * inv) << (8 * j);
-      *reinterpret_cast<uint32_t*>(q + static_cast<size_t>(row) * (k >> 1) + (c >> 1)) = w;
+      *reinterpret_cast<uint32_t*>(q + static_cast<size_t>(dst) * (k >> 1) + (c >> 1)) = w;
     }
     // the four blocks of the 16 lanes' atom as one word; blocks that pad the last K tile have b = 0
     uint32_t s = b << (8 * ((lane >> 2) & 3));
     s |= __shfl_xor_sync(0xffffffffu, s, 4);
     s |= __shfl_xor_sync(0xffffffffu, s, 8);
     const int g = c >> 5;
-    if ((lane & 15) == 0 && (g >> 2) < ka) *reinterpret_cast<uint32_t*>(sf + row_sf_off(row, g, ka)) = s;
+    if ((lane & 15) == 0 && (g >> 2) < ka) *reinterpret_cast<uint32_t*>(sf + row_sf_off(dst, g, ka)) = s;
   }
 }
 
@@ -212,14 +213,14 @@ dequant_mxfp4_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ 
 }
 
 template <int IN>
-cudaError_t launch_quant(bool vec, const void* x, long long ldx, int m, int k, int ka, void* q, void* sf, const void* src_rows,
-                         const void* total_rows, int gather, cudaStream_t st) {
+cudaError_t launch_quant(bool vec, const void* x, long long ldx, int m, int k, int ka, void* q, void* sf, const void* dst_rows,
+                         int topk, cudaStream_t st) {
   const int segs = (ka * 128 + SEG - 1) / SEG;
   const long long units = static_cast<long long>(m) * segs, blocks = (units + QUANT_WARPS - 1) / QUANT_WARPS;
   if (units > 0x7FFFFFF0ll) return cudaErrorInvalidValue;
   return launch_dep(vec ? quant_mxfp4_kernel<IN, true> : quant_mxfp4_kernel<IN, false>, dim3(static_cast<unsigned>(blocks)),
                     dim3(QUANT_WARPS * 32), 0, st, x, ldx, m, k, ka, static_cast<uint8_t*>(q), static_cast<uint8_t*>(sf), segs,
-                    static_cast<const int*>(src_rows), static_cast<const int*>(total_rows), gather);
+                    static_cast<const int*>(dst_rows), topk);
 }
 
 }  // namespace
@@ -227,17 +228,17 @@ cudaError_t launch_quant(bool vec, const void* x, long long ldx, int m, int k, i
 
 extern "C" {
 
-int hb_quant_mxfp4(const void* x, int in_type, long long ldx, int m, int k, int ka, void* q, void* sf, const void* src_rows,
-                   const void* total_rows, int gather, void* stream) {
+int hb_quant_mxfp4(const void* x, int in_type, long long ldx, int m, int k, int ka, void* q, void* sf, const void* dst_rows, int topk,
+                   void* stream) {
   using namespace hb;
   if (m < 1 || k < 32 || k % 32 != 0 || ka != (k + 255) / 256 * 2) return 1;
   const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ldx % (in_type == kInF32 ? 4 : 8) == 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   switch (in_type) {
-    case kInBf16: e = launch_quant<kInBf16>(vec, x, ldx, m, k, ka, q, sf, src_rows, total_rows, gather, st); break;
-    case kInF16: e = launch_quant<kInF16>(vec, x, ldx, m, k, ka, q, sf, src_rows, total_rows, gather, st); break;
-    case kInF32: e = launch_quant<kInF32>(vec, x, ldx, m, k, ka, q, sf, src_rows, total_rows, gather, st); break;
+    case kInBf16: e = launch_quant<kInBf16>(vec, x, ldx, m, k, ka, q, sf, dst_rows, topk, st); break;
+    case kInF16: e = launch_quant<kInF16>(vec, x, ldx, m, k, ka, q, sf, dst_rows, topk, st); break;
+    case kInF32: e = launch_quant<kInF32>(vec, x, ldx, m, k, ka, q, sf, dst_rows, topk, st); break;
     default: return 1;
   }
   return e == cudaSuccess ? 0 : 2;

@@ -303,8 +303,8 @@ def pair_rows(ew: "ExpertWeights", max_rows: int) -> bool:
     """Whether the grouped GEMMs run on SM pairs over 256-row chunks (csrc/gemm_pair.cu): FP4 experts as soon as a chunk
     would otherwise be a 128-token tile, in geometries whose activation can be requantised in fc1's epilogue. One-CTA tiles /
     pairs, whole call: 512 experts, top 22, 1024-2688-1024, 129 tokens 603 / 511 us, 256 639 / 531, 904 867 / 560, 4096
-    1910 / 697; 64 experts, top 8, 2048-768-2048 (SwiGLU), 129 tokens 108 / 79, 256 124 / 89, 904 178 / 120, 4096 551 / 236. MXFP4: 664 / 508 and
-    1747 / 668 at 129 and 4096 tokens of the first, 121 / 90 and 535 / 227 of the second."""
+    1910 / 697; 64 experts, top 8, 2048-768-2048 (SwiGLU), 129 tokens 108 / 79, 256 124 / 89, 904 178 / 120, 4096 551 / 236. MXFP4, 4096
+    tokens: 1747 / 668 and 535 / 227 (662 and 225 with the activations quantised by pair)."""
     return (ew.fmt in ("nvfp4", "mxfp4") and max_rows > 128 and ew.act in ("swiglu", "relu2") and ew.inter % 64 == 0
             and ew.n1 % 128 == 0 and ew.fc2_rows % 128 == 0)
 
@@ -365,7 +365,7 @@ def experts_forward(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, e
                                      ew.inter, y.data_ptr(), y.stride(0), None, gemm.EPI_STORE, start.data_ptr(),
                                      cnt.data_ptr(), max_rows, st.data_ptr(), 0, 0, bn_hint, *tl, nv.stream()), "hb_gemm_grouped")
     elif ew.fmt == "mxfp4":
-        q1 = mxfp4.quantize(x, src_rows=src, total_rows=total, rows=rows_cap, gather=True)
+        q1 = mxfp4.quantize_pairs(x, pos, topk, rows_cap)
         if pairs:
             q2 = mxfp4.empty(rows_cap, ew.inter, dev)
             epi = gemm.EPI_SILU_MUL_QUANT if ew.act == "swiglu" else gemm.EPI_RELU2_QUANT
@@ -377,7 +377,7 @@ def experts_forward(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, e
             nv.check(lib.hb_gemm_grouped(4, ew.fc1.q.data_ptr(), q1.q.data_ptr(), ew.fc1.sf.data_ptr(), q1.sf.data_ptr(), e, n1,
                                          rows_cap, h, h1.data_ptr(), h1.stride(0), None, epi1, start.data_ptr(), cnt.data_ptr(),
                                          max_rows, st.data_ptr(), ew.fc1.ka, q1.ka, bn_hint, *tl, nv.stream()), "hb_gemm_grouped")
-            q2 = mxfp4.quantize(h1, src_rows=src, total_rows=total)      # (the padding between segments stays as it is)
+            q2 = mxfp4.quantize_pairs(h1, pos, 0, rows_cap)
         nv.check(lib.hb_gemm_grouped(4, ew.fc2.q.data_ptr(), q2.q.data_ptr(), ew.fc2.sf.data_ptr(), q2.sf.data_ptr(), e, h_out,
                                      rows_cap, ew.inter, y.data_ptr(), y.stride(0), None, gemm.EPI_STORE, start.data_ptr(),
                                      cnt.data_ptr(), max_rows, st.data_ptr(), ew.fc2.ka, q2.ka, bn_hint, *tl, nv.stream()),

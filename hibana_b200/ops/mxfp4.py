@@ -20,7 +20,7 @@ from .nvfp4 import e2m1_codes, e2m1_values, swizzle_blocks, unswizzle_sf
 BLOCK = 32
 NAN_SCALE = 255
 
-nv.register("hb_quant_mxfp4", [nv.P, nv.I, nv.L, nv.I, nv.I, nv.I, nv.P, nv.P, nv.P, nv.P, nv.I, nv.P])
+nv.register("hb_quant_mxfp4", [nv.P, nv.I, nv.L, nv.I, nv.I, nv.I, nv.P, nv.P, nv.P, nv.I, nv.P])
 nv.register("hb_dequant_mxfp4", [nv.P, nv.P, nv.I, nv.I, nv.I, nv.P, nv.I, nv.P])
 
 IN_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -133,34 +133,39 @@ def empty(m: int, k: int, device: torch.device) -> Mxfp4Tensor:
     return Mxfp4Tensor(*_alloc(m, k, device), m, k)
 
 
-def quantize(x: torch.Tensor, *, src_rows: torch.Tensor | None = None, total_rows: torch.Tensor | None = None,
-             rows: int | None = None, gather: bool = False) -> Mxfp4Tensor:
-    """Rows [M, K] (bf16, fp16 or fp32; any row stride, K a multiple of 32) -> MXFP4.
-
-    `src_rows` (int32 [rows], CUDA only; the expert-sorted buffers of a mixture-of-experts layer): rows with a negative entry,
-    and rows from `total_rows` (int32 [1]) on, are left unwritten; with `gather` output row r is quantised from
-    x[src_rows[r]]."""
+def quantize(x: torch.Tensor) -> Mxfp4Tensor:
+    """Rows [M, K] (bf16, fp16 or fp32; any row stride, K a multiple of 32) -> MXFP4."""
     m, k = _check(x)
-    if src_rows is None:
-        if gather or total_rows is not None or (rows is not None and rows != m):
-            raise ValueError("MXFP4: gather, total_rows and rows go with src_rows")
-    else:
-        m = m if rows is None else rows
-        if not x.is_cuda or not 0 <= m <= src_rows.numel() or (not gather and m > x.shape[0]):
-            raise ValueError(f"MXFP4: {m} rows of {x.shape[0]} by {src_rows.numel()} row numbers on {x.device}")
-        for v in (src_rows, total_rows):
-            if v is not None and (v.dtype != torch.int32 or v.device != x.device or not v.is_contiguous() or v.numel() < 1):
-                raise ValueError("MXFP4: row numbers and counts are contiguous int32 tensors on the rows' device")
     if nv.use_native(x):
         q, sf = _alloc(m, k, x.device)
         if m:
-            with nv.on_device(x):
-                nv.check(nv.lib().hb_quant_mxfp4(x.data_ptr(), IN_TYPES[x.dtype], x.stride(0), m, k, k_atoms(k),
-                                                 q.data_ptr(), sf.data_ptr(), nv.ptr(src_rows), nv.ptr(total_rows),
-                                                 int(gather), nv.stream()), "hb_quant_mxfp4")
+            _launch(x, m, k, q, sf, None, 0)
         return Mxfp4Tensor(q, sf, m, k)
     packed, sfb = quantize_ref(x)
     return Mxfp4Tensor(packed, swizzle_blocks(sfb, k_atoms(k)), m, k)
+
+
+def _launch(x, m, k, q, sf, pos, topk) -> None:
+    with nv.on_device(x):
+        nv.check(nv.lib().hb_quant_mxfp4(x.data_ptr(), IN_TYPES[x.dtype], x.stride(0), m, k, k_atoms(k), q.data_ptr(),
+                                         sf.data_ptr(), nv.ptr(pos), topk, nv.stream()), "hb_quant_mxfp4")
+
+
+def quantize_pairs(x: torch.Tensor, pos: torch.Tensor, topk: int, rows: int) -> Mxfp4Tensor:
+    """Into the expert-sorted buffer of a mixture-of-experts layer (CUDA only), [rows, K]: pair p of `pos` (int32, one number a
+    token and expert, below `rows`) becomes row pos[p], from x[p // topk] or, with topk 0, from x[pos[p]]. Pairs with a negative
+    number are left out; the other rows are left unwritten."""
+    m, k = _check(x)
+    n = pos.numel()
+    if not x.is_cuda or pos.dtype != torch.int32 or pos.device != x.device or not pos.is_contiguous():
+        raise ValueError("MXFP4: row numbers are a contiguous int32 tensor on the rows' CUDA device")
+    if topk < 0 or (n != m * topk if topk else rows > m) or rows < 0:
+        raise ValueError(f"MXFP4: {n} row numbers (top {topk}) of {rows} rows do not fit {m} rows")
+    nv.use_native(x)
+    out = empty(rows, k, x.device)
+    if n and rows:
+        _launch(x, n, k, out.q, out.sf, pos, topk)
+    return out
 
 
 def quantize_weight(w: torch.Tensor) -> Mxfp4Tensor:

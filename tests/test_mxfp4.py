@@ -162,14 +162,19 @@ def test_every_code_and_scale_gpu():
 
 
 @pytest.mark.gpu
-def test_quantiser_rows_of_a_sorted_buffer_gpu():
-    x = _rows(9, 160).cuda()
-    src = torch.tensor([4, -1, 0, 8, -1, 4, 2, 1], dtype=torch.int32, device="cuda")
-    total = torch.tensor([6], dtype=torch.int32, device="cuda")
-    t = mxfp4.quantize(x, src_rows=src, total_rows=total, rows=8, gather=True)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_quantiser_into_a_sorted_buffer_gpu(dtype):
+    x = _rows(3, 160).to(dtype).cuda()
+    pos = torch.tensor([4, -1, 0, 130, 2, 11], dtype=torch.int32, device="cuda")
     plain = mxfp4.quantize(x)
-    for r, s in ((0, 4), (2, 0), (3, 8), (5, 4)):
-        assert torch.equal(t.q[r], plain.q[s]) and torch.equal(t.scales()[r], plain.scales()[s])
+    t = mxfp4.quantize_pairs(x, pos, 2, 131)
+    for p, r in enumerate(pos.tolist()):
+        assert r < 0 or (torch.equal(t.q[r], plain.q[p // 2]) and torch.equal(t.scales()[r], plain.scales()[p // 2]))
+    wide = torch.zeros(131, 160, dtype=dtype, device="cuda")
+    wide[[4, 0, 130, 2, 11]] = x[[0, 1, 1, 2, 2]]
+    u = mxfp4.quantize_pairs(wide, pos, 0, 131)
+    for r in (4, 0, 130, 2, 11):
+        assert torch.equal(u.q[r], t.q[r]) and torch.equal(u.scales()[r], t.scales()[r])
 
 
 def _product_case(m, n, k, seed=0):
@@ -255,20 +260,15 @@ def test_product_in_a_graph_and_on_another_stream_gpu():
 
 
 def test_row_number_refusals_cpu():
-    x = torch.randn(4, 64).bfloat16()
-    idx = torch.arange(4, dtype=torch.int32)
-    for kw in ({"gather": True}, {"rows": 5}, {"total_rows": idx[:1]}, {"src_rows": idx}):      # (row numbers are for the GPU)
-        with pytest.raises(ValueError):
-            mxfp4.quantize(x, **kw)
+    with pytest.raises(ValueError):                    # (expert-sorted buffers are the GPU's)
+        mxfp4.quantize_pairs(torch.randn(4, 64).bfloat16(), torch.arange(4, dtype=torch.int32), 1, 4)
 
 
 @pytest.mark.gpu
 def test_row_number_refusals_gpu():
     x = torch.randn(4, 64, device="cuda").bfloat16()
-    idx = torch.arange(8, dtype=torch.int32, device="cuda")
-    for kw in ({"src_rows": idx.long()}, {"src_rows": idx.cpu()}, {"src_rows": idx[::2]}, {"src_rows": idx, "rows": 5},
-               {"src_rows": idx, "rows": 9, "gather": True}, {"src_rows": idx, "total_rows": idx[:1].long()}):
+    pos = torch.arange(8, dtype=torch.int32, device="cuda")
+    for args in ((pos.long(), 2, 8), (pos.cpu(), 2, 8), (pos[::2], 1, 4), (pos, 1, 8), (pos, 3, 8), (pos, 0, 5), (pos, -1, 4), (pos, 2, -1)):
         with pytest.raises(ValueError):
-            mxfp4.quantize(x, **kw)
-    q = mxfp4.quantize(x, src_rows=idx.flip(0)[4:].contiguous(), rows=4, gather=True)
-    assert torch.equal(q.dequantize(), mxfp4.quantize(x.flip(0).contiguous()).dequantize())
+            mxfp4.quantize_pairs(x, *args)
+    assert mxfp4.quantize_pairs(x[:0], pos[:0], 2, 0).rows == 0
