@@ -270,7 +270,9 @@ def experts_ref(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, ew: E
             e = int(ids[ti, k]) - id_base
             if e < e_lo or e >= e_lo + e_n:
                 continue
-            h1 = (xf[ti] @ w1[e].t()).to(torch.bfloat16).float() if ew.act != "swiglu" else xf[ti] @ w1[e].t()
+            h1 = xf[ti] @ w1[e].t()
+            if ew.act != "swiglu" and ew.fmt != "mxfp4":     # (MXFP4: rounded once, behind the activation, as the kernels do)
+                h1 = h1.to(torch.bfloat16).float()
             mid = _act(h1, ew.act).to(torch.bfloat16)
             if ew.fmt == "nvfp4":
                 q, sfb = nvfp4.quantize_ref(mid.view(1, -1), ew.fc2_in_scale)
