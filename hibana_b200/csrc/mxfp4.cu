@@ -9,9 +9,9 @@
 // Packed values are row-major (low nibble first); scale bytes go to the 128 x 4 blocks that tcgen05.cp moves into TMEM, four
 // of a row (128 elements) being one 32-bit word.
 //
-// Bound by bytes: 2 (bf16) or 4 in and 17/32 out per element. Four lanes share a block: each holds eight elements (one or two
-// 16-byte loads), the maximum takes two shuffles, and sixteen lanes' scales make the word of an atom. A warp works on 1024
-// elements of a row at a time, all of its loads in flight at once.
+// Bound by bytes: 2 (bf16) or 4 in and 17/32 out per element. Two lanes share a block: each holds sixteen elements (one or two 32-byte
+// loads), the maximum takes one shuffle, and eight lanes' scales make the word of an atom. A warp works on 1024 elements of a row at a
+// time, all of its loads in flight at once.
 //
 // Measured, from memory: 2048 x 17408 bf16 quantised in 21.7 us (90 MB, 4.2 TB/s: bound by the instructions of the maxima and the packing),
 // back in 13.6; 17408 x 5120 fp32 68.6 (404 MB, 5.9 TB/s) and 61.8; one row of 5120 2.8 and 2.2, launch and latency.
@@ -28,56 +28,63 @@ constexpr int QUANT_WARPS = 4;
 constexpr int SEG = 1024;              // elements of a row per warp: 4 steps of 256
 enum InType : int { kInBf16 = 0, kInF16 = 1, kInF32 = 2 };
 
-// Eight consecutive elements as floats; VEC: 16-byte aligned.
-template <int IN, bool VEC>
-struct Raw8 {
-  uint4 a, b;
+// Sixteen consecutive elements, half a block; ALIGN: bytes that their address and the rows' pitch are multiples of (32, 16 or the type's).
+template <int IN, int ALIGN>
+struct Raw16 {
+  static constexpr int WORDS = IN == kInF32 ? 16 : 8;
+  uint32_t w[WORDS];
   __device__ __forceinline__ void load(const void* x, long long i) {
-    if constexpr (VEC) {
-      const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(x) + i * (IN == kInF32 ? 4 : 2));
-      a = ld_step(p);
-      if constexpr (IN == kInF32) b = ld_step(p + 1);
-    } else {
-      uint32_t w[8];
-      if constexpr (IN == kInF32) {
+    const uint8_t* at = static_cast<const uint8_t*>(x) + i * (IN == kInF32 ? 4 : 2);
+    if constexpr (ALIGN == 32) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = ld_step(static_cast<const uint32_t*>(x) + i + j);
-        b = make_uint4(w[4], w[5], w[6], w[7]);
-      } else {
-        const unsigned short* p = static_cast<const unsigned short*>(x) + i;
+      for (int j = 0; j < WORDS; j += 8)
+        asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(w[j]), "=r"(w[j + 1]), "=r"(w[j + 2]), "=r"(w[j + 3]), "=r"(w[j + 4]), "=r"(w[j + 5]), "=r"(w[j + 6]),
+                       "=r"(w[j + 7])
+                     : "l"(at + j * 4));
+    } else if constexpr (ALIGN == 16) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = static_cast<uint32_t>(ld_step(p + 2 * j)) | static_cast<uint32_t>(ld_step(p + 2 * j + 1)) << 16;
+      for (int j = 0; j < WORDS; j += 4) {
+        const uint4 v = ld_step(reinterpret_cast<const uint4*>(at + j * 4));
+        w[j] = v.x; w[j + 1] = v.y; w[j + 2] = v.z; w[j + 3] = v.w;
       }
-      a = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < WORDS; ++j) {
+        if constexpr (IN == kInF32) {
+          w[j] = ld_step(reinterpret_cast<const uint32_t*>(at) + j);
+        } else {
+          const unsigned short* p = reinterpret_cast<const unsigned short*>(at) + 2 * j;
+          w[j] = static_cast<uint32_t>(ld_step(p)) | static_cast<uint32_t>(ld_step(p + 1)) << 16;
+        }
+      }
     }
   }
-  // Bits of the largest magnitude as a float (an order in which NaN comes last). bf16 words are compared two at a time: with every
-  // element compared by itself the kernel was bound by those instructions (2048 x 17408: 24 us for 14 us of bytes).
-  __device__ __forceinline__ uint32_t top(const float (&f)[8]) const {
-    if constexpr (IN == kInBf16) {
-      const uint32_t m = __vmaxu2(__vmaxu2(a.x & 0x7FFF7FFFu, a.y & 0x7FFF7FFFu), __vmaxu2(a.z & 0x7FFF7FFFu, a.w & 0x7FFF7FFFu));
-      return max(m << 16, m & 0xFFFF0000u);
-    }
+  // Bits of the largest magnitude as a float (an order in which NaN comes last), 16-bit numbers compared two at a time.
+  __device__ __forceinline__ uint32_t top() const {
     uint32_t m = 0;
+    if constexpr (IN == kInF32) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(f[j]) & 0x7FFFFFFFu);
-    return m;
+      for (int j = 0; j < WORDS; ++j) m = max(m, w[j] & 0x7FFFFFFFu);
+      return m;
+    }
+#pragma unroll
+    for (int j = 0; j < WORDS; ++j) m = __vmaxu2(m, w[j] & 0x7FFF7FFFu);
+    if constexpr (IN == kInBf16) return max(m << 16, m & 0xFFFF0000u);
+    const uint32_t h = max(m >> 16, m & 0xFFFFu);
+    return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(h))));
   }
-  __device__ __forceinline__ void floats(float (&f)[8]) const {
-    if constexpr (IN == kInBf16) {
-      unpack8(a, f);
-    } else if constexpr (IN == kInF16) {
-      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-        f[2 * j] = t.x;
-        f[2 * j + 1] = t.y;
-      }
+  __device__ __forceinline__ void pair(int j, float& lo, float& hi) const {      // elements 2j, 2j + 1
+    if constexpr (IN == kInF32) {
+      lo = __uint_as_float(w[2 * j]);
+      hi = __uint_as_float(w[2 * j + 1]);
+    } else if constexpr (IN == kInBf16) {
+      lo = bf16_lo(w[j]);
+      hi = bf16_hi(w[j]);
     } else {
-      const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(w[j]);
+      const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+      lo = t.x;
+      hi = t.y;
     }
   }
 };
@@ -85,8 +92,8 @@ struct Raw8 {
 // dst_rows (may be null; the expert-sorted buffers of a mixture-of-experts layer, m pairs of a token and one of its topk experts): pair r
 // goes to row dst_rows[r], of token r / topk or, with topk 0, of the same row of x; a negative entry leaves the pair out. The other rows
 // of the buffers (most of them, with few tokens: every expert's segment is padded to 128) are not touched.
-template <int IN, bool VEC>
-__global__ void __launch_bounds__(QUANT_WARPS * 32, IN == kInF32 ? 9 : 16)
+template <int IN, int ALIGN>
+__global__ void __launch_bounds__(QUANT_WARPS * 32, IN == kInF32 ? 9 : 12)
 quant_mxfp4_kernel(const void* __restrict__ x, long long ldx, int m, int k, int ka, uint8_t* __restrict__ q,
                    uint8_t* __restrict__ sf, int segs, const int* __restrict__ dst_rows, int topk) {
   grid_dep_wait(x, dst_rows);
@@ -103,37 +110,36 @@ quant_mxfp4_kernel(const void* __restrict__ x, long long ldx, int m, int k, int 
     in_row = topk > 0 ? row / topk : dst;
   }
   const long long base = in_row * ldx;
-  const int k0 = seg * SEG + lane * 8;
-  Raw8<IN, VEC> raw[4];
+  constexpr int STEP = 512, STEPS = SEG / STEP;
+  const int k0 = seg * SEG + lane * 16;
+  Raw16<IN, ALIGN> raw[STEPS];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (k0 + i * 256 < k) raw[i].load(x, base + k0 + i * 256);
+  for (int i = 0; i < STEPS; ++i)
+    if (k0 + i * STEP < k) raw[i].load(x, base + k0 + i * STEP);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int c = k0 + i * 256;                   // (k is a multiple of 32: a block is there as a whole or not at all)
-    if (seg * SEG + i * 256 >= ka * 128) break;   // uniform
-    float f[8];
-    uint32_t top = 0;
-    if (c < k) {
-      raw[i].floats(f);
-      top = raw[i].top(f);
-    }
+  for (int i = 0; i < STEPS; ++i) {
+    const int c = k0 + i * STEP;                   // (k is a multiple of 32: a block is there as a whole or not at all)
+    if (seg * SEG + i * STEP >= ka * 128) break;   // uniform
+    uint32_t top = c < k ? raw[i].top() : 0u;
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
     float inv;
     const uint32_t b = mx_scale(top, inv);
     if (c < k) {
-      uint32_t w = 0;
+      uint32_t w[2] = {0, 0};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w |= e2m1x2(f[2 * j] * inv, f[2 * j + 1] * inv) << (8 * j);
-      *reinterpret_cast<uint32_t*>(q + static_cast<size_t>(dst) * (k >> 1) + (c >> 1)) = w;
+      for (int j = 0; j < 8; ++j) {
+        float lo, hi;
+        raw[i].pair(j, lo, hi);
+        w[j >> 2] |= e2m1x2(lo * inv, hi * inv) << (8 * (j & 3));
+      }
+      *reinterpret_cast<uint2*>(q + static_cast<size_t>(dst) * (k >> 1) + (c >> 1)) = make_uint2(w[0], w[1]);
     }
-    // the four blocks of the 16 lanes' atom as one word; blocks that pad the last K tile have b = 0
-    uint32_t s = b << (8 * ((lane >> 2) & 3));
+    // the four blocks of the eight lanes' atom as one word; blocks that pad the last K tile have b = 0
+    uint32_t s = b << (8 * ((lane >> 1) & 3));
+    s |= __shfl_xor_sync(0xffffffffu, s, 2);
     s |= __shfl_xor_sync(0xffffffffu, s, 4);
-    s |= __shfl_xor_sync(0xffffffffu, s, 8);
     const int g = c >> 5;
-    if ((lane & 15) == 0 && (g >> 2) < ka) *reinterpret_cast<uint32_t*>(sf + row_sf_off(dst, g, ka)) = s;
+    if ((lane & 7) == 0 && (g >> 2) < ka) *reinterpret_cast<uint32_t*>(sf + row_sf_off(dst, g, ka)) = s;
   }
 }
 
@@ -213,12 +219,13 @@ dequant_mxfp4_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ 
 }
 
 template <int IN>
-cudaError_t launch_quant(bool vec, const void* x, long long ldx, int m, int k, int ka, void* q, void* sf, const void* dst_rows,
+cudaError_t launch_quant(int align, const void* x, long long ldx, int m, int k, int ka, void* q, void* sf, const void* dst_rows,
                          int topk, cudaStream_t st) {
   const int segs = (ka * 128 + SEG - 1) / SEG;
   const long long units = static_cast<long long>(m) * segs, blocks = (units + QUANT_WARPS - 1) / QUANT_WARPS;
   if (units > 0x7FFFFFF0ll) return cudaErrorInvalidValue;
-  return launch_dep(vec ? quant_mxfp4_kernel<IN, true> : quant_mxfp4_kernel<IN, false>, dim3(static_cast<unsigned>(blocks)),
+  auto kern = align == 32 ? quant_mxfp4_kernel<IN, 32> : align == 16 ? quant_mxfp4_kernel<IN, 16> : quant_mxfp4_kernel<IN, 0>;
+  return launch_dep(kern, dim3(static_cast<unsigned>(blocks)),
                     dim3(QUANT_WARPS * 32), 0, st, x, ldx, m, k, ka, static_cast<uint8_t*>(q), static_cast<uint8_t*>(sf), segs,
                     static_cast<const int*>(dst_rows), topk);
 }
@@ -232,13 +239,14 @@ int hb_quant_mxfp4(const void* x, int in_type, long long ldx, int m, int k, int 
                    void* stream) {
   using namespace hb;
   if (m < 1 || k < 32 || k % 32 != 0 || ka != (k + 255) / 256 * 2) return 1;
-  const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ldx % (in_type == kInF32 ? 4 : 8) == 0;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(x) | static_cast<uintptr_t>(ldx * (in_type == kInF32 ? 4 : 2));
+  const int align = at % 32 == 0 ? 32 : at % 16 == 0 ? 16 : 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   switch (in_type) {
-    case kInBf16: e = launch_quant<kInBf16>(vec, x, ldx, m, k, ka, q, sf, dst_rows, topk, st); break;
-    case kInF16: e = launch_quant<kInF16>(vec, x, ldx, m, k, ka, q, sf, dst_rows, topk, st); break;
-    case kInF32: e = launch_quant<kInF32>(vec, x, ldx, m, k, ka, q, sf, dst_rows, topk, st); break;
+    case kInBf16: e = launch_quant<kInBf16>(align, x, ldx, m, k, ka, q, sf, dst_rows, topk, st); break;
+    case kInF16: e = launch_quant<kInF16>(align, x, ldx, m, k, ka, q, sf, dst_rows, topk, st); break;
+    case kInF32: e = launch_quant<kInF32>(align, x, ldx, m, k, ka, q, sf, dst_rows, topk, st); break;
     default: return 1;
   }
   return e == cudaSuccess ? 0 : 2;
