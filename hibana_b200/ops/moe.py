@@ -498,8 +498,9 @@ def layer_forward(x: torch.Tensor, router: torch.Tensor, ew: ExpertWeights, topk
     if shared is not None and (shared.shape != (t, ew.fc2_rows) or shared.dtype != torch.bfloat16):
         raise ValueError(f"layer_forward: bf16 shared rows {(t, ew.fc2_rows)} expected, got {shared.dtype} {tuple(shared.shape)}")
     w1 = ew.fc1 if isinstance(ew.fc1, torch.Tensor) else ew.fc1.q
+    dev = x.get_device()
     for other in (router, rx, w1, sel_bias, shared):
-        if other is not None and other.device != x.device:
+        if other is not None and other.get_device() != dev:
             raise ValueError("layer_forward: operands on different devices")
     few = t <= FEW_TOKENS and few_tokens_ok(ew, topk)
     if not nv.use_native(x):
