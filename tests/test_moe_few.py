@@ -381,3 +381,18 @@ def test_grouped_mxfp4_experts_step_by_step_gpu(t, act):
     # are that near, 128 a row and expert: one row in sixteen), counted here, not bounded.
     off = (got - want).abs() <= 2.0 ** -8 * 1.01 * (size + want.abs()) + 1e-6
     assert off.all(dim=1).float().mean() >= 0.9 and nv.read_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t,e,k,h,inter,act,fmt", [
+    (1, 12, 12, 4640, 1664, "relu2", "nvfp4"),        # two rounds of fc1, the second sparse; more scales than tensor memory holds
+    (1, 12, 12, 512, 1664, "relu2", "mxfp4"),
+    (2, 20, 10, 256, 2560, "relu2", "bf16"),
+    (1, 11, 11, 4640, 1664, "relu2", "nvfp4"),        # one round
+    (4, 24, 12, 128, 896, "swiglu", "mxfp4"),         # three or four rounds
+])
+def test_rounds_of_the_first_product_gpu(t, e, k, h, inter, act, fmt):
+    ew, x, rx, router, bias, sh = _case(t, e, h, act, fmt, inter, seed=8, h_out=128)
+    got = moe.layer_forward(x.cuda(), router.cuda(), ew.to("cuda"), k, shared=sh.cuda())
+    _check(got, *_exact(ew, x, rx, router, k, False, bias, 1.0, sh))
+    assert nv.read_status() == 0

@@ -272,3 +272,19 @@ def test_row_number_refusals_gpu():
         with pytest.raises(ValueError):
             mxfp4.quantize_pairs(x, *args)
     assert mxfp4.quantize_pairs(x[:0], pos[:0], 2, 0).rows == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_quantiser_alignments_gpu(dtype):
+    """Rows that start on 32-, 16- and 4- or 2-byte boundaries, at every length of the last piece of a row."""
+    for k in (32, 480, 512, 992, 1024, 1056, 1568):
+        base = _rows(6, k + 64, seed=k).to(dtype)
+        for offset in (0, 1, 4, 8, 16):
+            for pad in (0, 1, 4, 8, 16):
+                view = torch.as_strided(base.cuda().flatten(), (5, k), (k + pad, 1), offset)
+                want = mxfp4.quantize(torch.as_strided(base.flatten(), (5, k), (k + pad, 1), offset))
+                got = mxfp4.quantize(view)
+                assert torch.equal(got.q.cpu(), want.q) and torch.equal(got.scales().cpu(), want.scales()), (k, offset, pad)
+                # blocks that pad the last K tile read as zero
+                assert not mxfp4.unswizzle_sf(got.sf, 5, got.ka * 4)[:, k // 32:].any()
