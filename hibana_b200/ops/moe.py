@@ -1,8 +1,9 @@
 """Mixture-of-experts forward: route -> plan -> (gather | quantise) -> grouped fc1 (+act) -> grouped fc2 -> combine.
 
 `ExpertWeights` holds all experts of a layer stacked: fc1 [E, 2I, H] with gate/up rows interleaved pairwise
-(SwiGLU) or [E, I, H] (ReLU^2), fc2 [E, H, I]; bf16 or NVFP4 (one per-tensor scale per expert). The grouped GEMMs
-are the grouped mode of the tcgen05 GEMM. With expert parallelism a rank plans only its own expert range
+(SwiGLU) or [E, I, H] (ReLU^2), fc2 [E, H, I]; bf16, NVFP4 (one per-tensor scale per expert) or MXFP4. The grouped GEMMs
+are the grouped mode of the tcgen05 GEMM. `layer_forward` is a whole layer, router included; up to 16 tokens it does without
+the plan, the gather and the combine (csrc/moe_few.cu). With expert parallelism a rank plans only its own expert range
 [e_lo, e_lo + e_n) and produces a partial sum (replicated-activation EP; the all-to-all variant lives in
 parallel/ep.py). Reference: hibana/model/flashnext/moe.py:68-192, hibana/model/nemotron/moe.py:349-566,
 hibana/kernels/w3_moe.py:194 (reference), hibana/kernels/csrc/w3_gemm.cu:640-1300.
@@ -468,7 +469,10 @@ def _few_sizes(kind: int, tokens: int, experts: int, topk: int, hidden: int, int
 
 def _rows16(x: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     """Rows that 16-byte loads can read: as they are, or copied."""
-    if x is None or (x.stride(-1) == 1 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0):
+    if x is None:
+        return x
+    rows, cols = x.stride()
+    if cols == 1 and rows % 8 == 0 and x.data_ptr() % 16 == 0:
         return x
     return x.clone(memory_format=torch.contiguous_format)
 
@@ -483,9 +487,10 @@ def layer_forward(x: torch.Tensor, router: torch.Tensor, ew: ExpertWeights, topk
     (logits; both products) that stream the chosen experts' weights once and read the activations in bf16, whatever the experts' format; more
     tokens, and layers `few_tokens_ok` does not cover, take `linear_bf16`, `route` and `experts_forward` (which quantises
     activations for FP4 experts)."""
-    if x.dim() != 2 or x.dtype != torch.bfloat16 or x.shape[1] != ew.hidden:
-        raise ValueError(f"layer_forward: bf16 rows of width {ew.hidden} expected, got {x.dtype} {tuple(x.shape)}")
-    t, e = x.shape[0], ew.experts
+    shape, e = x.shape, ew.experts
+    if len(shape) != 2 or x.dtype != torch.bfloat16 or shape[1] != ew.hidden:
+        raise ValueError(f"layer_forward: bf16 rows of width {ew.hidden} expected, got {x.dtype} {tuple(shape)}")
+    t = shape[0]
     rx = x if route_x is None else route_x
     if router.dim() != 2 or router.shape[0] != e or router.dtype != torch.bfloat16:
         raise ValueError(f"layer_forward: a bf16 router of {e} rows expected, got {router.dtype} {tuple(router.shape)}")
@@ -538,9 +543,11 @@ def _few_launch(kind, x, rx, router, ew, topk, score, sel_bias, shared, out) -> 
     if kind == 0:
         w1, w2 = (fc1.data_ptr(), None, None, 0), (fc2.data_ptr(), None, None, 0)
     else:
-        w1, w2 = ((w.q.data_ptr(), w.sf.data_ptr(), w.gscale.data_ptr() if kind == 1 else None, w.sf.shape[1]) for w in (fc1, fc2))
+        w1 = (fc1.q.data_ptr(), fc1.sf.data_ptr(), fc1.gscale.data_ptr() if kind == 1 else None, fc1.sf.shape[1])
+        w2 = (fc2.q.data_ptr(), fc2.sf.data_ptr(), fc2.gscale.data_ptr() if kind == 1 else None, fc2.sf.shape[1])
+    h_out = out.shape[1]
     nv.check(nv.lib().hb_moe_few(kind, x.data_ptr(), x.stride(0), rx.data_ptr(), rx.stride(0), router.data_ptr(),
-                                 router.stride(0), router.shape[1], nv.ptr(sel_bias), t, e, topk, *score, h, i, out.shape[1],
+                                 router.stride(0), router.shape[1], nv.ptr(sel_bias), t, e, topk, *score, h, i, h_out,
                                  int(ew.act == "swiglu"), *w1, *w2, nv.ptr(shared), 0 if shared is None else shared.stride(0),
-                                 out.data_ptr(), out.stride(0), ws.data_ptr(), nv.device_state(dev).status.data_ptr(),
+                                 out.data_ptr(), h_out, ws.data_ptr(), nv.device_state(dev).status.data_ptr(),
                                  nv.stream()), "hb_moe_few", launches=3)
