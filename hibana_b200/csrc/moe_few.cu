@@ -29,9 +29,9 @@
 // part of the experts, and add up through distributed shared memory in order.
 //
 // Measured (us a call among others, weights from memory; in brackets route / fc1 / fc2 on their own, and the time of the bytes at the copy
-// rate): 512 experts, 2560-640 SwiGLU, MXFP4, top 10: 1 token 25 (4.0 / 14 / 15.5; 4.4), 16 tokens 78 (4.4 / 50 / 36; 56); 512
-// experts, 1024-2688 squared ReLU, NVFP4, top 22, router over 4096: 4 tokens 60 (5.8 / 33 / 34; 40); 64 experts, 2048-768 SwiGLU, bf16,
-// top 8: 7 tokens 69 (3.5 / 48 / 31; 56). The products stream 5 to 6.6 TB/s while they stream. Bound by what happens before the first
+// rate): 512 experts, 2560-640 SwiGLU, MXFP4, top 10: 1 token 23 (4.0 / 14 / 15.5; 4.4), 16 tokens 75 (4.4 / 50 / 36; 56); 512
+// experts, 1024-2688 squared ReLU, NVFP4, top 22, router over 4096: 4 tokens 59 (5.8 / 33 / 34; 40); 64 experts, 2048-768 SwiGLU, bf16,
+// top 8: 7 tokens 70 (3.5 / 48 / 31; 56). The products stream 5 to 6.6 TB/s while they stream. Bound by what happens before the first
 // weights can be named and between kernels: logits 4, top-k and plan 4, first tiles 2 each, from fc1's last tile to fc2's first 5, the
 // cluster's sums 3. fc2 runs on the clusters that fit (80 to 120 of 148 SMs: 120 with clusters of six on 20 output blocks). Fetching the
 // first of W2 into L2 from fc1's last tiles on made 16 tokens 2 us slower.
