@@ -726,7 +726,8 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
     const bool resident = SECOND || SFB_COL + k_tiles * T::ATOMS * 4 <= TMEM_COLS;
     if constexpr (T::kFp4) {
       tc_fence_after();
-      if (resident && set == 0 && ok && elect_one()) {
+      // (not by a CTA without a unit: nobody there waits for these copies, and it would leave while they run)
+      if (resident && set == 0 && u0 < units && ok && elect_one()) {
         for (int at = 0; at < (SECOND ? 1 : k_tiles * T::ATOMS); ++at)
           tmem_cp_32x128b_x4(tmem + SFB_COL + at * 4, make_desc_sf(xsf_addr + at * 512));
         tc_commit(sfb_full);
