@@ -666,9 +666,10 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
   const int streams = two ? 2 : 1, S = two ? p.stages & ~1 : p.stages;
   // With two streams units go in pairs, K tile by K tile: the first's stages are the even ones, the second's the odd ones.
   const uint32_t ring_addr = __shfl_sync(0xffffffffu, smem_u32(ring), 0), xsf_addr = __shfl_sync(0xffffffffu, smem_u32(xsf), 0);
+  int issued = 0, alone = 0x7FFFFFFF;         // warp 0: tiles asked for so far; from `alone` on every other place is left out
   if (warp == 0) {
     // ---- weights: the whole warp walks the loop (waits included), one elected lane issues
-    int i = 0, s = 0, alone = 0x7FFFFFFF;      // place in the ring's order; from `alone` on every other one is left out
+    int i = 0, s = 0;                         // place in the ring's order
     uint32_t phase = 1;                       // (the first round finds every stage free)
     bool ok = true;
     for (int u = u0; u < units && ok; u += streams * stride) {
@@ -708,11 +709,7 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
         }
       }
     }
-    if (!ok && lane == 0) {                   // bounded wait for the copies still in flight: none may land after the CTA has gone
-      volatile int ignore = 0;
-      for (int j = max(i - S, 0); j < i; ++j)
-        if (j < alone || (j & 1) == 0) mbar_wait(&full[j % S], (j / S) & 1, &ignore, nullptr, kTimeoutDrain);
-    }
+    issued = i;
     __syncwarp();
   } else if (warp == 1 || (two && warp == 3)) {
     // ---- products
@@ -900,15 +897,19 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
       }
     }
   }
-  if constexpr (!SECOND) {
-    if (*abort && tid == 0) {                 // (the rows of x as well)
-      volatile int ignore = 0;
-      mbar_wait(x_full, 0, &ignore, nullptr, kTimeoutDrain);
-    }
-  }
   __syncwarp();
   tc_fence_before();
   __syncthreads();
+  if (*abort) {                               // (one answer for the whole CTA: behind the barrier nobody raises it any more)
+    // bounded wait for the copies still in flight, whichever warp gave up: none may land after the CTA has gone
+    if (tid == 0) {
+      volatile int ignore = 0;
+      if constexpr (!SECOND) mbar_wait(x_full, 0, &ignore, nullptr, kTimeoutDrain);
+      for (int j = max(issued - S, 0); j < issued; ++j)
+        if (j < alone || (j & 1) == 0) mbar_wait(&full[j % S], (j / S) & 1, &ignore, nullptr, kTimeoutDrain);
+    }
+    __syncthreads();
+  }
   if (warp == 1) tmem_dealloc(tmem, TMEM_COLS);
   if constexpr (SECOND) {
     const int n_out = p.tokens * 128;

@@ -18,6 +18,16 @@ def test_resident_scales_are_copied_only_where_a_unit_waits_for_them_cpu():
     assert "u0 < units" in guard and "elect_one()" in guard
 
 
+def test_a_wait_that_gave_up_anywhere_drains_every_copy_cpu():
+    """Any warp can raise the abort flag, so what drains the copies asks for it behind a barrier, does not depend on how the
+    loader's own waits ended, and has the rest of the CTA wait for it."""
+    tail = SOURCE[SOURCE.index("} else if (SECOND && warp >= 12)"):SOURCE.index("tmem_dealloc(tmem, TMEM_COLS)")]
+    assert SOURCE.count("kTimeoutDrain") == tail.count("kTimeoutDrain") == 2            # x's rows and the ring's tiles, in one place
+    before, drain = tail.split("if (*abort) {")
+    assert before.rstrip().splitlines()[-1].strip() == "__syncthreads();"
+    assert drain.index("mbar_wait(x_full") < drain.index("__syncthreads();") and drain.index("mbar_wait(&full[") < drain.index("__syncthreads();")
+
+
 def _layer(e, h, inter, act, fmt, seed):
     g = torch.Generator().manual_seed(seed)
     n1 = 2 * inter if act == "swiglu" else inter
