@@ -234,8 +234,8 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) moe_few_route_kernel(const _
         const int k = (b0 + i * ROUTE_WARPS) * 32 + t * 8;
         wa[i] = wb[i] = va[i] = vb[i] = make_uint4(0, 0, 0, 0);
         if (k < p.route_k) {
-          wa[i] = __ldg(reinterpret_cast<const uint4*>(ra + k));
-          wb[i] = __ldg(reinterpret_cast<const uint4*>(rb + k));
+          wa[i] = ld_step(reinterpret_cast<const uint4*>(ra + k));
+          wb[i] = ld_step(reinterpret_cast<const uint4*>(rb + k));
           va[i] = ld_step(reinterpret_cast<const uint4*>(xa + k));
           if (two) vb[i] = ld_step(reinterpret_cast<const uint4*>(xb + k));
         }
@@ -799,7 +799,7 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
       tc_fence_after();
       const int entry = u / tiles, tile = u - entry * tiles, n = plan.count[entry], expert = plan.expert[entry];
       const float* gp = SECOND ? p.gs2 : p.gs1;
-      const float gs = KIND == kGemmNvfp4 ? __ldg(gp + expert) : 1.f;
+      const float gs = KIND == kGemmNvfp4 ? ld_step(gp + expert) : 1.f;
       const int row = tile * 128 + row_in;
 #pragma unroll 1
       for (int c = 0; c < n; ++c) {
