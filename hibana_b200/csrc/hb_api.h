@@ -100,10 +100,11 @@ int hb_quant_nvfp4_rows(const void* x, long long ldx, int m, int k, int ka, cons
                         int mode, const void* src_rows, const void* total_rows, void* stream);
 int hb_norm_quant_nvfp4(const void* x, void* residual, const void* w, float eps, int gemma, int m, int k, int ka,
                         const void* gscale, void* q, void* sf, void* normed, void* stream);
-// MXFP4 (mxfp4.cu): x of type 0 bf16, 1 fp16, 2 fp32; ka = 2 * ceil(k / 256) scale atoms per row block. src_rows / total_rows
-// (may be null): rows with a negative entry and rows from *total_rows on stay unwritten; gather: row r comes from src_rows[r].
-int hb_quant_mxfp4(const void* x, int in_type, long long ldx, int m, int k, int ka, void* q, void* sf, const void* dst_rows, int topk,
-                   void* stream);
+// MXFP4 (mxfp4.cu): x of type 0 bf16, 1 fp16, 2 fp32; ka = 2 * ceil(k / 256) scale atoms per row block. dst_rows (may be null: row r
+// goes to row r): pair r goes to row dst_rows[r], from row r / topk of x or, with topk 0, from row dst_rows[r]; pairs whose entry is not
+// in [0, dst_count) are left out, rows that no pair names stay unwritten.
+int hb_quant_mxfp4(const void* x, int in_type, long long ldx, int m, int k, int ka, void* q, void* sf, const void* dst_rows,
+                   int dst_count, int topk, void* stream);
 int hb_dequant_mxfp4(const void* q, const void* sf, int m, int k, int ka, void* out, int out_type, void* stream);
 int hb_quant_fp8_static(const void* x, long long n, const void* scale, void* q, void* stream);
 int hb_quant_fp8_rows(const void* x, int m, int k, void* q, void* scales, void* stream);

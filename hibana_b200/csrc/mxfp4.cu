@@ -91,12 +91,12 @@ struct Raw16 {
 };
 
 // dst_rows (may be null; the expert-sorted buffers of a mixture-of-experts layer, m pairs of a token and one of its topk experts): pair r
-// goes to row dst_rows[r], of token r / topk or, with topk 0, of the same row of x; a negative entry leaves the pair out. The other rows
-// of the buffers (most of them, with few tokens: every expert's segment is padded to 128) are not touched.
+// goes to row dst_rows[r], of token r / topk or, with topk 0, of the same row of x; an entry that is negative or not below dst_count (rows
+// of the buffers, and with topk 0 of x) leaves the pair out. The other rows of the buffers (most of them, with few tokens: every expert's segment is padded to 128) are not touched.
 template <int IN, int ALIGN>
 __global__ void __launch_bounds__(QUANT_WARPS * 32, IN == kInF32 ? 9 : 12)
 quant_mxfp4_kernel(const void* __restrict__ x, long long ldx, int m, int k, int ka, uint8_t* __restrict__ q,
-                   uint8_t* __restrict__ sf, int segs, const int* __restrict__ dst_rows, int topk) {
+                   uint8_t* __restrict__ sf, int segs, const int* __restrict__ dst_rows, int dst_count, int topk) {
   grid_dep_wait(x, dst_rows);
   grid_dep_launch();      // behind the wait: a grouped GEMM that follows reads the routing plan at once (see launch_dep)
   const uint32_t unit = blockIdx.x * QUANT_WARPS + (threadIdx.x >> 5);      // (the launch keeps it below 2^31)
@@ -107,7 +107,7 @@ quant_mxfp4_kernel(const void* __restrict__ x, long long ldx, int m, int k, int 
   int dst = row;
   if (dst_rows != nullptr) {
     dst = dst_rows[row];
-    if (dst < 0) return;
+    if (static_cast<uint32_t>(dst) >= static_cast<uint32_t>(dst_count)) return;
     in_row = topk > 0 ? row / topk : dst;
   }
   const long long base = in_row * ldx;
@@ -221,14 +221,14 @@ dequant_mxfp4_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ 
 
 template <int IN>
 cudaError_t launch_quant(int align, const void* x, long long ldx, int m, int k, int ka, void* q, void* sf, const void* dst_rows,
-                         int topk, cudaStream_t st) {
+                         int dst_count, int topk, cudaStream_t st) {
   const int segs = (ka * 128 + SEG - 1) / SEG;
   const long long units = static_cast<long long>(m) * segs, blocks = (units + QUANT_WARPS - 1) / QUANT_WARPS;
   if (units > 0x7FFFFFF0ll) return cudaErrorInvalidValue;
   auto kern = align == 32 ? quant_mxfp4_kernel<IN, 32> : align == 16 ? quant_mxfp4_kernel<IN, 16> : quant_mxfp4_kernel<IN, 0>;
   return launch_dep(kern, dim3(static_cast<unsigned>(blocks)),
                     dim3(QUANT_WARPS * 32), 0, st, x, ldx, m, k, ka, static_cast<uint8_t*>(q), static_cast<uint8_t*>(sf), segs,
-                    static_cast<const int*>(dst_rows), topk);
+                    static_cast<const int*>(dst_rows), dst_count, topk);
 }
 
 }  // namespace
@@ -236,8 +236,8 @@ cudaError_t launch_quant(int align, const void* x, long long ldx, int m, int k, 
 
 extern "C" {
 
-int hb_quant_mxfp4(const void* x, int in_type, long long ldx, int m, int k, int ka, void* q, void* sf, const void* dst_rows, int topk,
-                   void* stream) {
+int hb_quant_mxfp4(const void* x, int in_type, long long ldx, int m, int k, int ka, void* q, void* sf, const void* dst_rows,
+                   int dst_count, int topk, void* stream) {
   using namespace hb;
   if (m < 1 || k < 32 || k % 32 != 0 || ka != (k + 255) / 256 * 2) return 1;
   const uintptr_t at = reinterpret_cast<uintptr_t>(x) | static_cast<uintptr_t>(ldx * (in_type == kInF32 ? 4 : 2));
@@ -245,9 +245,9 @@ int hb_quant_mxfp4(const void* x, int in_type, long long ldx, int m, int k, int 
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   switch (in_type) {
-    case kInBf16: e = launch_quant<kInBf16>(align, x, ldx, m, k, ka, q, sf, dst_rows, topk, st); break;
-    case kInF16: e = launch_quant<kInF16>(align, x, ldx, m, k, ka, q, sf, dst_rows, topk, st); break;
-    case kInF32: e = launch_quant<kInF32>(align, x, ldx, m, k, ka, q, sf, dst_rows, topk, st); break;
+    case kInBf16: e = launch_quant<kInBf16>(align, x, ldx, m, k, ka, q, sf, dst_rows, dst_count, topk, st); break;
+    case kInF16: e = launch_quant<kInF16>(align, x, ldx, m, k, ka, q, sf, dst_rows, dst_count, topk, st); break;
+    case kInF32: e = launch_quant<kInF32>(align, x, ldx, m, k, ka, q, sf, dst_rows, dst_count, topk, st); break;
     default: return 1;
   }
   return e == cudaSuccess ? 0 : 2;

@@ -20,7 +20,7 @@ from .nvfp4 import e2m1_codes, e2m1_values, swizzle_blocks, unswizzle_sf
 BLOCK = 32
 NAN_SCALE = 255
 
-nv.register("hb_quant_mxfp4", [nv.P, nv.I, nv.L, nv.I, nv.I, nv.I, nv.P, nv.P, nv.P, nv.I, nv.P])
+nv.register("hb_quant_mxfp4", [nv.P, nv.I, nv.L, nv.I, nv.I, nv.I, nv.P, nv.P, nv.P, nv.I, nv.I, nv.P])
 nv.register("hb_dequant_mxfp4", [nv.P, nv.P, nv.I, nv.I, nv.I, nv.P, nv.I, nv.P])
 
 IN_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -139,22 +139,22 @@ def quantize(x: torch.Tensor) -> Mxfp4Tensor:
     if nv.use_native(x):
         q, sf = _alloc(m, k, x.device)
         if m:
-            _launch(x, m, k, q, sf, None, 0)
+            _launch(x, m, k, q, sf, None, m, 0)
         return Mxfp4Tensor(q, sf, m, k)
     packed, sfb = quantize_ref(x)
     return Mxfp4Tensor(packed, swizzle_blocks(sfb, k_atoms(k)), m, k)
 
 
-def _launch(x, m, k, q, sf, pos, topk) -> None:
+def _launch(x, m, k, q, sf, pos, rows, topk) -> None:
     with nv.on_device(x):
         nv.check(nv.lib().hb_quant_mxfp4(x.data_ptr(), IN_TYPES[x.dtype], x.stride(0), m, k, k_atoms(k), q.data_ptr(),
-                                         sf.data_ptr(), nv.ptr(pos), topk, nv.stream()), "hb_quant_mxfp4")
+                                         sf.data_ptr(), nv.ptr(pos), rows, topk, nv.stream()), "hb_quant_mxfp4")
 
 
 def quantize_pairs(x: torch.Tensor, pos: torch.Tensor, topk: int, rows: int) -> Mxfp4Tensor:
     """Into the expert-sorted buffer of a mixture-of-experts layer (CUDA only), [rows, K]: pair p of `pos` (int32, one number a
-    token and expert, below `rows`) becomes row pos[p], from x[p // topk] or, with topk 0, from x[pos[p]]. Pairs with a negative
-    number are left out; the other rows are left unwritten."""
+    token and expert) becomes row pos[p], from x[p // topk] or, with topk 0, from x[pos[p]]. Pairs whose number is negative or
+    not below `rows` are left out, and rows that no pair names are left unwritten. A row that two pairs name holds either's."""
     m, k = _check(x)
     n = pos.numel()
     if not x.is_cuda or pos.dtype != torch.int32 or pos.device != x.device or not pos.is_contiguous():
@@ -164,7 +164,7 @@ def quantize_pairs(x: torch.Tensor, pos: torch.Tensor, topk: int, rows: int) -> 
     nv.use_native(x)
     out = empty(rows, k, x.device)
     if n and rows:
-        _launch(x, n, k, out.q, out.sf, pos, topk)
+        _launch(x, n, k, out.q, out.sf, pos, rows, topk)
     return out
 
 

@@ -288,3 +288,24 @@ def test_quantiser_alignments_gpu(dtype):
                 assert torch.equal(got.q.cpu(), want.q) and torch.equal(got.scales().cpu(), want.scales()), (k, offset, pad)
                 # blocks that pad the last K tile read as zero
                 assert not mxfp4.unswizzle_sf(got.sf, 5, got.ka * 4)[:, k // 32:].any()
+
+
+def test_row_numbers_are_bounded_in_the_kernel_cpu():
+    """Row numbers live on the device, so the kernel itself keeps them inside the buffers, ahead of any use."""
+    from pathlib import Path
+    source = (Path(mxfp4.__file__).parent.parent / "csrc" / "mxfp4.cu").read_text()
+    body = source[source.index("dst = dst_rows[row];"):]
+    assert body.splitlines()[1].strip() == "if (static_cast<uint32_t>(dst) >= static_cast<uint32_t>(dst_count)) return;"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("topk", [0, 2])
+def test_row_numbers_past_the_buffer_are_left_out_gpu(topk):
+    x = _rows(6, 160).cuda()
+    n = 6 * topk if topk else 7
+    pos = torch.tensor([4, 6, -1, 2 ** 31 - 1, 1, -2 ** 31, 5, 7, 2 ** 20, 0, 128, 3][:n], dtype=torch.int32, device="cuda")
+    plain = mxfp4.quantize(x)
+    out = mxfp4.quantize_pairs(x, pos, topk, 6)
+    for p, r in enumerate(pos.tolist()):
+        src = p // topk if topk else r
+        assert not 0 <= r < 6 or (torch.equal(out.q[r], plain.q[src]) and torch.equal(out.scales()[r], plain.scales()[src]))
