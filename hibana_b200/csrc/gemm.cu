@@ -1007,7 +1007,7 @@ cudaError_t launch_t(const GemmArgs& a, DevParams& p, dim3 grid, const CUtensorM
   using C = Cfg<KIND, BN>;
   constexpr int K_ELEMS = is_fp4(KIND) ? 256 : KIND == kGemmFp8 ? 128 : 64;      // of a K tile
   static bool attr_done[kMaxDevices] = {};
-  static int max_clusters[9] = {0, 0, 0, 0, 0, 0, 0, 0, 0};   // co-resident clusters per cluster size (0 = unknown)
+  static DeviceCounts<9> max_clusters;                        // co-resident clusters per cluster size
   if (bool& done = attr_done[device_index()]; !done) {
     cudaError_t e = cudaFuncSetAttribute(gemm_kernel<KIND, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          C::SMEM_BYTES);
@@ -1027,7 +1027,7 @@ cudaError_t launch_t(const GemmArgs& a, DevParams& p, dim3 grid, const CUtensorM
     const int tiles = grid.x * grid.y;
     for (; splits > 1; --splits) {
       if (splits > 1 && (splits - 1) * ((p.k_tiles + splits - 1) / splits) >= p.k_tiles) continue;
-      if (max_clusters[splits] == 0) {
+      const int room = max_clusters.get(device_index(), splits, [splits] {
         cudaLaunchConfig_t q = {};
         q.gridDim = dim3(1, 1, splits);
         q.blockDim = dim3(NUM_THREADS);
@@ -1037,12 +1037,12 @@ cudaError_t launch_t(const GemmArgs& a, DevParams& p, dim3 grid, const CUtensorM
         qa[0].val.clusterDim.x = 1; qa[0].val.clusterDim.y = 1; qa[0].val.clusterDim.z = splits;
         q.attrs = qa; q.numAttrs = 1;
         int n = 0;
-        if (cudaOccupancyMaxActiveClusters(&n, gemm_kernel<KIND, BN>, &q) != cudaSuccess || n < 1) {
+        if (cudaOccupancyMaxActiveClusters(&n, gemm_kernel<KIND, BN>, &q) != cudaSuccess) {
           (void)cudaGetLastError();
           n = -1;
         }
-        max_clusters[splits] = n;
-      }
+        return n;
+      });
       // The query counts one CTA per SM for a kernel that allocates tensor memory. Two do run where shared memory and
       // tensor memory hold two (BN <= 64): with 148 slots assumed, K was cut half as often as the chip has room for. A
       // negative split count asks for the wider tiles' limit at every width: the same cuts, so the same order of sums,
@@ -1050,7 +1050,6 @@ cudaError_t launch_t(const GemmArgs& a, DevParams& p, dim3 grid, const CUtensorM
       // For 64-token tiles the second CTA of an SM pays from 512 elements of K per split on: 64 rows, bf16, 4096 x 1024 in 8
       // splits of 128 9.2 us, 4 of 256 7.9; 4096 x 2048 in 8 of 256 10.4, 4 of 512 9.2; 5120 x 3072 in 6 of 512 11.1, 3 of 1024 11.9;
       // 7168 x 5120 with and without the second CTA 15.5 and 23.1.
-      const int room = max_clusters[splits];
       const bool two = BN < 64 || (BN == 64 && (p.k_tiles + splits - 1) / splits * K_ELEMS >= 512);
       if ((two && a.splits > 0 ? 2 * room : room) >= tiles) break;
     }

@@ -693,10 +693,11 @@ cudaError_t gemm_pair_launch(const GemmArgs& a, cudaStream_t stream) {
     return std::min(n, resident_clusters<kGemmMxfp4, kEpiSiluMulQuant, true>());
   };
   const bool mx = a.kind == kGemmMxfp4;
-  static int known[2][kMaxDevices] = {};      // + 1
-  int& slot = known[mx][device_index()];
-  if (slot == 0) slot = (mx ? resident_mx() : resident_nv()) + 1;
-  const int resident = slot - 1;
+  static DeviceCounts<2> known;
+  const int resident = known.get(device_index(), mx, [&] {
+    const int n = mx ? resident_mx() : resident_nv();
+    return n < 1 ? -1 : n;                    // (a set-up that failed is tried again)
+  });
   if (resident < 1) return cudaErrorInvalidConfiguration;
   const bool grouped = a.grp_cnt != nullptr;
   // tokens are the A side here; a grouped call names its weights first

@@ -12,11 +12,11 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include "device_counts.h"
+
 namespace hb {
 
-constexpr int kMaxDevices = 16;   // of a process: kernel attributes are set once on each
-
-// Current device, as the index of such a table.
+// Current device, as the index of a table of kMaxDevices entries (device_counts.h).
 inline int device_index() {
   int dev = 0;
   return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < kMaxDevices ? dev : kMaxDevices - 1;

@@ -941,8 +941,8 @@ moe_few_experts_kernel(const __grid_constant__ CUtensorMap tw, const __grid_cons
 // Clusters of `size` CTAs of the second kernel that the chip holds at once (0: none).
 template <int KIND>
 int resident(int size) {
-  static int known[MAX_CLUSTER + 1] = {};              // + 1
-  if (known[size] == 0) {
+  static DeviceCounts<MAX_CLUSTER + 1> known;
+  return known.get(device_index(), size, [size] {
     int n = 0;
     cudaLaunchConfig_t q = {};
     q.gridDim = dim3(size);
@@ -956,11 +956,10 @@ int resident(int size) {
     q.numAttrs = 1;
     if (cudaOccupancyMaxActiveClusters(&n, moe_few_experts_kernel<KIND, true>, &q) != cudaSuccess) {
       (void)cudaGetLastError();
-      n = 0;
+      n = -1;
     }
-    known[size] = n + 1;
-  }
-  return known[size] - 1;
+    return n;
+  });
 }
 
 template <int KIND>
