@@ -514,17 +514,22 @@ def layer_forward(x: torch.Tensor, router: torch.Tensor, ew: ExpertWeights, topk
     with nv.on_device(x):
         if t == 0:
             return torch.empty(0, ew.fc2_rows, dtype=torch.bfloat16, device=x.device)
+        # both forms: rows that 16-byte loads can read, a router whose rows are whole 16 bytes (zeros behind an odd width), a plain bias
+        x, shared = _rows16(x), _rows16(shared)
+        rx = x if route_x is None else route_x
+        pad = -router.shape[1] % 8
+        if pad:
+            rx, router = F.pad(rx, (0, pad)), F.pad(router, (0, pad))
+        rx, router = _rows16(rx), _rows16(router)
+        if sel_bias is not None:
+            sel_bias = sel_bias.contiguous()
         kind = _KINDS.get(ew.fmt, 0)
         most = _few_sizes(kind, t, e, topk, ew.hidden, ew.inter)[0] if few else 0       # (a wide layer's rows take several calls)
-        if most * 2 < t or router.shape[1] % 8:
+        if most * 2 < t:
             ids, w = route(gemm.linear_bf16(rx, router, epilogue=gemm.EPI_STORE_F32), topk, sigmoid=sigmoid, sel_bias=sel_bias,
                            renorm=renorm, scale=scale)
             return experts_forward(x, ids, w, ew, shared=shared)
         out = torch.empty(t, ew.fc2_rows, dtype=torch.bfloat16, device=x.device)
-        x, router, shared = _rows16(x), _rows16(router), _rows16(shared)
-        rx = x if route_x is None else _rows16(route_x)
-        if sel_bias is not None:
-            sel_bias = sel_bias.contiguous()
         score = (int(sigmoid), int(renorm), scale)
         if most >= t:
             _few_launch(kind, x, rx, router, ew, topk, score, sel_bias, shared, out)
