@@ -95,8 +95,9 @@ class EngineConfig:
     pdl: int = 2                           # programmatic dependent launch level (0 off, 1 GEMMs, 2 most kernels)
     overlap_rows: int = 64                 # up to this many rows a MoE layer's independent chains (shared expert,
                                            # latent projection) run on a side stream beside the routed experts; 0 = off
-    moe_few: bool = False                  # bf16 and NVFP4 MoE layers of up to 16 rows on one GPU run as one few-token layer
-                                           # (moe.layer_forward: activations unquantised); MXFP4 layers always do
+    moe_few: bool = False                  # bf16 and NVFP4 MoE layers of up to 16 rows (fewer, or none, in wide layers:
+                                           # moe.few_tokens_per_call) on one GPU run as one few-token layer
+                                           # (moe.layer_forward: activations not quantised to FP4); MXFP4 layers always do
     expert_budget: int = 0                 # > 0: decode-sized MoE calls read at most this many distinct experts
     expert_keep: int = 2                   # with a budget: choices of every row that are always honoured
     # observability

@@ -503,13 +503,13 @@ class MoeLayer:
 
     def _takes_few(self, rows: int) -> bool:
         """Whether a call of `rows` rows runs as one few-token layer (`moe.layer_forward`): MXFP4 experts always, the other
-        formats with `moe_few`. Off where the routing is edited between its kernels (`expert_budget`) and under
+        formats with `moe_few`, as far as the layer's width allows (`moe.few_tokens_per_call`). Off where the routing is edited between its kernels (`expert_budget`) and under
         `stable_numerics` (the form reads unquantised activations, so a request's tokens would depend on how many rows ran
         beside it)."""
         cfg, ew = cfgmod.current(), self.experts
-        return (0 < rows <= moe.FEW_TOKENS and (ew.fmt == "mxfp4" or cfg.moe_few) and self.ep_size == 1
-                and self.experts_w3 is None and cfg.expert_budget <= 0 and not cfg.stable_numerics
-                and moe.few_tokens_ok(ew, self.t.top_k))
+        return ((ew.fmt == "mxfp4" or cfg.moe_few) and self.ep_size == 1 and self.experts_w3 is None
+                and cfg.expert_budget <= 0 and not cfg.stable_numerics
+                and moe.few_tokens_per_call(ew, self.t.top_k, rows) > 0)
 
     def _forward_few(self, x, ctx) -> torch.Tensor:
         t = self.t

@@ -454,17 +454,44 @@ def few_tokens_ref(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, ew
 
 
 def few_tokens_ok(ew: ExpertWeights, topk: int) -> bool:
-    """Whether the few-token form covers a layer: bf16, NVFP4 or MXFP4 experts, at most 1024 of them and 32 a token, with
-    whole blocks (128 rows of FP4 weights and their scales) per expert and matrix."""
+    """Whether the few-token form covers a layer of any width: bf16, NVFP4 or MXFP4 experts, at most 1024 of them and 32 a token,
+    with whole blocks (128 rows of FP4 weights and their scales) per expert and matrix. How many rows it takes at a width:
+    `few_tokens_limit`; whether it is what a call gets: `few_tokens_per_call`."""
     rows, k = (8, 8) if ew.fmt == "bf16" else (128, 32)
     return (ew.fmt in _KINDS and ew.act in ("swiglu", "relu2") and ew.experts <= 1024 and topk <= 32 and ew.n1 % rows == 0
             and ew.fc2_rows % rows == 0 and ew.hidden % k == 0 and ew.inter % k == 0)
 
 
 @functools.lru_cache(maxsize=1024)
-def _few_sizes(kind: int, tokens: int, experts: int, topk: int, hidden: int, inter: int) -> tuple[int, int]:
-    """(most tokens of one call at this width, workspace bytes of a call of `tokens`)."""
-    return nv.lib().hb_moe_few_tokens(kind, hidden), nv.lib().hb_moe_few_ws(kind, tokens, experts, topk, hidden, inter)
+def few_tokens_limit(fmt: str, hidden: int) -> int:
+    """Most tokens of one call of the kernels at a width: their first product holds all of the rows' columns in shared memory, five
+    of digits a row for FP4 experts, beside a ring of at least two tiles of weights (csrc/moe_few.cu, `hb_moe_few_tokens`). 16 up to
+    3584 columns in MXFP4, 3328 in NVFP4 and 5120 in bf16, then fewer: at 4096, 5120, 6144, 8192, 12288 MXFP4 12, 9, 6, 6, 3 and NVFP4 12, 9,
+    6, 3, 0; bf16 0 from 5448 on."""
+    fp4, atoms = fmt != "bf16", {"mxfp4": 2, "nvfp4": 4, "bf16": 0}[fmt]
+    k_tiles, per_row, sf = -(-hidden // (256 if fp4 else 64)), 5 if fp4 else 1, atoms * 512
+    for t in range(FEW_TOKENS, 0, -1):
+        rows = -(-t * per_row // 16) * 16
+        held = 1024 + k_tiles * (rows * 128 + sf) + t * 640 + 22608 + 304      # alignment, rows and scales, candidates, plan, barriers
+        if (227 * 1024 - held) // (128 * 128 + sf) >= 2:
+            return t
+    return 0
+
+
+def few_tokens_per_call(ew: ExpertWeights, topk: int, tokens: int) -> int:
+    """Tokens that a call of the kernels takes where `layer_forward` of `tokens` rows has the few-token form, 0 where it has the
+    grouped one: more than FEW_TOKENS rows, a layer that `few_tokens_ok` does not cover, or one so wide that two calls would not do
+    (every call reads its experts' weights). The same on every device."""
+    if not 0 < tokens <= FEW_TOKENS or not few_tokens_ok(ew, topk):
+        return 0
+    most = few_tokens_limit(ew.fmt, ew.hidden)
+    return min(most, tokens) if 2 * most >= tokens else 0
+
+
+@functools.lru_cache(maxsize=1024)
+def _few_ws(kind: int, tokens: int, experts: int, topk: int, hidden: int, inter: int) -> int:
+    """Workspace bytes of a call."""
+    return nv.lib().hb_moe_few_ws(kind, tokens, experts, topk, hidden, inter)
 
 
 def _rows16(x: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -484,9 +511,10 @@ def layer_forward(x: torch.Tensor, router: torch.Tensor, ew: ExpertWeights, topk
 
     router bf16 [E, Hr]; its input rows are `route_x` [T, Hr] (a latent layer routes on the hidden rows) or x. Scores, top-k and
     weights as in `route`; `shared` [T, H_out] bf16 is added to the sum. Up to FEW_TOKENS tokens the layer is three kernels
-    (logits; both products) that stream the chosen experts' weights once and read the activations in bf16, whatever the experts' format; more
-    tokens, and layers `few_tokens_ok` does not cover, take `linear_bf16`, `route` and `experts_forward` (which quantises
-    activations for FP4 experts)."""
+    (logits; both products) that stream the chosen experts' weights once, whatever the experts' format, and a layer of
+    more than 3328 columns may be two such calls (`few_tokens_limit`). More tokens, layers `few_tokens_ok` does not cover and layers too wide
+    for two calls (`few_tokens_per_call` is 0) take `linear_bf16`, `route` and `experts_forward`, which quantises the activations of FP4
+    experts to their format."""
     shape, e = x.shape, ew.experts
     if len(shape) != 2 or x.dtype != torch.bfloat16 or shape[1] != ew.hidden:
         raise ValueError(f"layer_forward: bf16 rows of width {ew.hidden} expected, got {x.dtype} {tuple(shape)}")
@@ -507,10 +535,10 @@ def layer_forward(x: torch.Tensor, router: torch.Tensor, ew: ExpertWeights, topk
     for other in (router, rx, w1, sel_bias, shared):
         if other is not None and other.get_device() != dev:
             raise ValueError("layer_forward: operands on different devices")
-    few = t <= FEW_TOKENS and few_tokens_ok(ew, topk)
+    most = few_tokens_per_call(ew, topk, t)
     if not nv.use_native(x):
         ids, w = route_ref(rx.float() @ router.float().t(), topk, sigmoid=sigmoid, sel_bias=sel_bias, renorm=renorm, scale=scale)
-        return few_tokens_ref(x, ids, w, ew, shared) if few else experts_forward(x, ids, w, ew, shared=shared)
+        return few_tokens_ref(x, ids, w, ew, shared) if most else experts_forward(x, ids, w, ew, shared=shared)
     with nv.on_device(x):
         if t == 0:
             return torch.empty(0, ew.fc2_rows, dtype=torch.bfloat16, device=x.device)
@@ -523,15 +551,13 @@ def layer_forward(x: torch.Tensor, router: torch.Tensor, ew: ExpertWeights, topk
         rx, router = _rows16(rx), _rows16(router)
         if sel_bias is not None:
             sel_bias = sel_bias.contiguous()
-        kind = _KINDS.get(ew.fmt, 0)
-        most = _few_sizes(kind, t, e, topk, ew.hidden, ew.inter)[0] if few else 0       # (a wide layer's rows take several calls)
-        if most * 2 < t:
+        if not most:
             ids, w = route(gemm.linear_bf16(rx, router, epilogue=gemm.EPI_STORE_F32), topk, sigmoid=sigmoid, sel_bias=sel_bias,
                            renorm=renorm, scale=scale)
             return experts_forward(x, ids, w, ew, shared=shared)
         out = torch.empty(t, ew.fc2_rows, dtype=torch.bfloat16, device=x.device)
-        score = (int(sigmoid), int(renorm), scale)
-        if most >= t:
+        score, kind = (int(sigmoid), int(renorm), scale), _KINDS[ew.fmt]
+        if most == t:
             _few_launch(kind, x, rx, router, ew, topk, score, sel_bias, shared, out)
         else:
             for lo in range(0, t, most):
@@ -544,7 +570,7 @@ def _few_launch(kind, x, rx, router, ew, topk, score, sel_bias, shared, out) -> 
     t, dev = x.shape[0], x.device
     gemm.init_pdl()
     e, h, i, fc1, fc2 = ew.experts, ew.hidden, ew.inter, ew.fc1, ew.fc2
-    ws = torch.empty(_few_sizes(kind, t, e, topk, h, i)[1], dtype=torch.uint8, device=dev)
+    ws = torch.empty(_few_ws(kind, t, e, topk, h, i), dtype=torch.uint8, device=dev)
     if kind == 0:
         w1, w2 = (fc1.data_ptr(), None, None, 0), (fc2.data_ptr(), None, None, 0)
     else:
