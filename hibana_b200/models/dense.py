@@ -149,6 +149,15 @@ class DenseModel:
             h = comm.all_reduce(h)
         return norm_linear(h, res, norm_w, t.norm_eps, lin, epilogue=epilogue, requant=requant)
 
+    @staticmethod
+    def _requants_down(layer, rows: int, cuda: bool, fused: bool) -> bool:
+        """Whether gate / up hand NVFP4 activations to the down projection (`fused`: attention does so to o_proj). A checkpoint's
+        projections may have formats of their own."""
+        if layer.down.fmt != "nvfp4" or layer.down.calibrating:
+            return False
+        return fused or (cfgmod.current().fuse_epilogues and cuda and layer.gate_up.fmt == "nvfp4"
+                         and gemm.requant_ok(rows, layer.gate_up.out_features))
+
     def _row_parallel(self, lin, x, ctx):
         """Row-parallel projection; returns (partial, heap slot or None)."""
         comm = ctx.comm
@@ -237,9 +246,7 @@ class DenseModel:
                                          else att.view(att.shape[0], -1), ctx)
             # prefill-sized chunks requantise in the gate/up epilogue too (tokens on the 128-row side of the GEMM):
             # the bf16 activation [rows, intermediate] is never written
-            fuse_mlp = fuse or (cfgmod.current().fuse_epilogues and q.is_cuda and layer.down.fmt == "nvfp4"
-                                and not layer.down.calibrating and layer.gate_up.fmt == "nvfp4"
-                                and gemm.requant_ok(q.shape[0], layer.gate_up.out_features))
+            fuse_mlp = self._requants_down(layer, q.shape[0], q.is_cuda, fuse)
             act = self._reduce_norm_linear(h, slot, res, layer.post_norm, layer.gate_up, ctx,
                                            epilogue=gemm.EPI_SILU_MUL,
                                            requant=layer.down.input_scale if fuse_mlp else None)
