@@ -208,8 +208,8 @@ class DenseModel:
         """ids int64 [T]; kv = KvPool. Returns normed hidden states of ctx.sample_rows (or of all rows)."""
         t = self.target
         if (ctx.comm is not None and getattr(ctx.comm, "sp_rows", 0) and ctx.mode == "prefill"
-                and ctx.comm.sp_ok(ids.shape[0], t.hidden) and not self.layers[0].qkv.calibrating
-                and self.layers[0].qkv.fmt != "mxfp4"):          # the peer-memory chain carries bf16 and NVFP4 rows
+                and ctx.comm.sp_ok(ids.shape[0], t.hidden)      # (and what the peer-memory chain carries)
+                and all(lin.fmt in ("bf16", "nvfp4") and not lin.calibrating for lin in self.linears())):
             return self.forward_sp(ids, ctx, kv)
         res = basic.embedding(ids, self.embed)
         if ctx.comm is None and self.layers[0].qkv.takes_gemv(ids.shape[0]) and self.layers[0].o.w3 is None:

@@ -5,6 +5,8 @@ import pytest
 import torch
 
 from hibana_b200 import _native as nv
+from hibana_b200.cache.kv_pool import KvPool
+from hibana_b200.engine.context import PREFILL, ForwardContext
 from hibana_b200.engine.executor import Executor
 from hibana_b200.engine.request import SamplingParams
 from hibana_b200.models.dense import DenseModel
@@ -39,6 +41,53 @@ def test_only_an_nvfp4_down_projection_is_handed_nvfp4_rows_cpu():
             assert got == (fmt == "nvfp4" and (fused or other == "nvfp4")), (fmt, other, fused)
         layer.down.calibrating = True
         assert not DenseModel._requants_down(layer, 4, True, True)
+
+
+class _Ranks:
+    """A communicator of one rank that offers the sequence-parallel chain."""
+    sp_rows, sp_hidden = 256, 256
+
+    def sp_ok(self, rows, hidden):
+        return True
+
+    def fits(self, rows, hidden):
+        return False
+
+    def all_reduce(self, x):
+        return x
+
+
+class _Chain(Exception):
+    pass
+
+
+def _prefill(model):
+    """Whether a prefill runs the sequence-parallel chain."""
+    t = model.target
+    pool = KvPool(model.kv_layers, 64, t.kv_heads, t.head_dim, device="cpu")
+    ctx = ForwardContext(PREFILL, torch.arange(6, dtype=torch.int32), torch.arange(1, 7, dtype=torch.int32),
+                         torch.arange(1, 7, dtype=torch.int32).view(1, 6), torch.tensor([6], dtype=torch.int32),
+                         q_indptr=torch.tensor([0, 6], dtype=torch.int32), max_rows=6, max_ctx_host=6, comm=_Ranks())
+
+    def chain(*args):
+        raise _Chain
+    model.forward_sp = chain
+    try:
+        out = model.forward(torch.arange(6), ctx, pool)
+    except _Chain:
+        return True
+    assert torch.isfinite(out.float()).all()
+    return False
+
+
+def test_the_sequence_parallel_chain_takes_layers_it_can_carry_cpu():
+    assert _prefill(_mixed({})) and _prefill(_mixed({"qkv": "bf16", "down": "bf16"}))
+    for part in ("qkv", "o", "gate_up", "down"):
+        assert not _prefill(_mixed({part: "mxfp4"}))
+        assert not _prefill(_mixed({}, per_layer={1: {part: "mxfp4"}}))
+    model = _mixed({"qkv": "bf16"})
+    model.layers[1].gate_up.calibrating = True           # (its range is recorded by the plain forward)
+    assert not _prefill(model)
 
 
 @pytest.mark.gpu
