@@ -212,7 +212,8 @@ class DenseModel:
                 and all(lin.fmt in ("bf16", "nvfp4") and not lin.calibrating for lin in self.linears())):
             return self.forward_sp(ids, ctx, kv)
         res = basic.embedding(ids, self.embed)
-        if ctx.comm is None and self.layers[0].qkv.takes_gemv(ids.shape[0]) and self.layers[0].o.w3 is None:
+        if (ctx.comm is None and self.layers[0].qkv.takes_gemv(ids.shape[0]) and self.layers[0].o.w3 is None
+                and all(lin.fmt == "nvfp4" for layer in self.layers for lin in (layer.o, layer.down))):
             return self._forward_few_rows(res, ctx, kv)
         h: Optional[torch.Tensor] = None
         slot = None

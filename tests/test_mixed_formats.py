@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from hibana_b200 import _native as nv
+from hibana_b200 import config as cfgmod
 from hibana_b200.cache.kv_pool import KvPool
 from hibana_b200.engine.context import PREFILL, ForwardContext
 from hibana_b200.engine.executor import Executor
@@ -97,3 +98,17 @@ def test_nvfp4_attention_beside_another_mlp_gpu(down, gate_up):
     model = _mixed({"qkv": "nvfp4", "o": "nvfp4", "gate_up": gate_up, "down": down}, "cuda")
     eager = _run(model)
     assert all(len(e) == 4 for e in eager) and _run(model, graphs=True) == eager and nv.read_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("part,fmt,layer", [("down", "mxfp4", 0), ("o", "bf16", 1), ("down", "bf16", 1), ("qkv", "mxfp4", 1), ("gate_up", "bf16", 0)])
+def test_few_row_decode_of_mixed_layers_gpu(part, fmt, layer):
+    """The few-row decode path (setting `gemv`) hands NVFP4 rows to o_proj and down, so it runs where all of those are NVFP4."""
+    model = _mixed({}, "cuda", {layer: {part: fmt}})
+    with cfgmod.using(gemv=True):
+        ran = []
+        whole = model._forward_few_rows
+        model._forward_few_rows = lambda *a: ran.append(1) or whole(*a)
+        eager = _run(model)
+        assert all(len(e) == 4 for e in eager) and bool(ran) == (part in ("qkv", "gate_up"))
+        assert _run(model, graphs=True) == eager and nv.read_status() == 0
