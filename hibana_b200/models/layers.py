@@ -468,6 +468,7 @@ class MoeLayer:
         return out
 
     experts_w3 = None      # optional 3-bit decode copy of the routed experts (attach_w3)
+    calibrating = False    # the routed rows are being collected (weights/calibrate_model.py): only the grouped form shows them
 
     def attach_w3(self, fc1=None, fc2=None) -> int:
         """3-bit decode copy of this rank's routed experts (int3, groups of 64, dequantisation fused into the grouped
@@ -507,7 +508,7 @@ class MoeLayer:
         `stable_numerics` (the form reads unquantised activations, so a request's tokens would depend on how many rows ran
         beside it)."""
         cfg, ew = cfgmod.current(), self.experts
-        return ((ew.fmt == "mxfp4" or cfg.moe_few) and self.ep_size == 1 and self.experts_w3 is None
+        return ((ew.fmt == "mxfp4" or cfg.moe_few) and self.ep_size == 1 and self.experts_w3 is None and not self.calibrating
                 and cfg.expert_budget <= 0 and not cfg.stable_numerics
                 and moe.few_tokens_per_call(ew, self.t.top_k, rows) > 0)
 

@@ -129,11 +129,15 @@ class ExpertCovariances:
                 cov._add(name, x, ids, weights, ew, kw.get("id_base", 0))
             return cov._original(x, ids, weights, ew, **kw)
         moe_ops.experts_forward = forward
+        for layer in self.layers.values():        # (the few-token form routes inside its kernels)
+            layer.calibrating = True
         return self
 
     def __exit__(self, *exc) -> None:
         from ..ops import moe as moe_ops
         moe_ops.experts_forward = self._original
+        for layer in self.layers.values():
+            layer.calibrating = False
 
 
 def fit_experts(model, ecov: ExpertCovariances, *, min_rows: int = 32, log=None) -> tuple[dict, list]:

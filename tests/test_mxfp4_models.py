@@ -224,3 +224,19 @@ def test_decoders_gpu(fmt, few):
             eager = _tokens(gpu, prompts, 10)
             assert _tokens(gpu, prompts, 10, use_graphs=True) == eager
             assert all(len(e) == 10 for e in eager) and nv.read_status() == 0
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4", "bf16"])
+def test_calibration_sees_the_rows_of_short_prompts_cpu(fmt):
+    """Chunks of up to sixteen rows count like any others: every (token, choice) pair, once."""
+    from hibana_b200.weights import calibrate_model as cm
+    t = scaled(tiny_hybrid_moe(), weight_format=fmt, expert_ffn=128, mtp_layers=0, mtp_depth=0)
+    model = HybridModel(t, "cpu", seed=0)
+    samples = _prompts(t.vocab, 3, 9) + _prompts(t.vocab, 1, 40)
+    with cfgmod.using(moe_few=True):
+        cov = cm.capture(model, samples, max_batch=1)
+    layers = cm.expert_layers(model)
+    assert layers and set(cov.experts.rows) == set(layers)
+    for name, layer in layers.items():
+        assert int(cov.experts.rows[name].sum()) == sum(map(len, samples)) * t.top_k
+        assert not layer.calibrating
