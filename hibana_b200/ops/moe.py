@@ -312,15 +312,26 @@ def pair_rows(ew: "ExpertWeights", max_rows: int) -> bool:
             and ew.n1 % 128 == 0 and ew.fc2_rows % 128 == 0)
 
 
+def check_grouped(ew: "ExpertWeights") -> None:
+    """Refuses experts that the grouped products do not tile: every matrix of an expert has a multiple of 128 rows, and columns in
+    multiples of 32 (FP4), 64 (3-bit) or 8 (bf16)."""
+    k = {"bf16": 8, "w3": 64}.get(ew.fmt, 32)
+    if ew.n1 % 128 or ew.fc2_rows % 128 or ew.hidden % k or ew.inter % k:
+        raise ValueError(f"{ew.fmt} experts of {ew.n1} x {ew.hidden} and {ew.fc2_rows} x {ew.inter}: the grouped products take rows in "
+                         f"multiples of 128 and columns in multiples of {k}")
+
+
 def experts_forward(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, ew: ExpertWeights, *,
                     shared: Optional[torch.Tensor] = None, e_lo: int = 0, e_n: Optional[int] = None,
                     id_base: int = 0) -> torch.Tensor:
     """x [T, H] bf16, ids / weights [T, k] -> [T, H_out] bf16 (sum of the routed experts (+ shared)). `ew` holds
     the experts `id_base` .. `id_base + ew.experts - 1` of the numbering `ids` use (an expert-parallel rank keeps a
-    range); of those, only [e_lo, e_lo + e_n) run. Pairs routed elsewhere add nothing."""
+    range); of those, only [e_lo, e_lo + e_n) run. Pairs routed elsewhere add nothing. On a GPU the experts' matrices have whole tiles
+    (`check_grouped`)."""
     e_n = ew.experts if e_n is None else e_n
     if not nv.use_native(x):
         return experts_ref(x, ids, weights, ew, shared, e_lo, e_n, id_base)
+    check_grouped(ew)
     lib = nv.lib()
     t, h = x.shape
     topk = ids.shape[1]

@@ -71,3 +71,42 @@ def test_strided_arguments_gpu(fmt, t):
     got = moe.layer_forward(x.t().contiguous().t(), router.t().contiguous().t(), ew, 3, sigmoid=True, sel_bias=bias,
                             shared=shared.t().contiguous().t(), route_x=rx.t().contiguous().t())
     assert torch.equal(got, want) and nv.read_status() == 0
+
+
+# format, act, hidden, inter, output columns
+UNTILED = [("mxfp4", "swiglu", 128, 96, 128), ("mxfp4", "relu2", 128, 128, 64), ("nvfp4", "relu2", 128, 192, 128), ("nvfp4", "swiglu", 144, 64, 128),
+           ("bf16", "swiglu", 48, 24, 48)]
+
+
+@pytest.mark.parametrize("fmt,act,h,inter,h_out", UNTILED)
+def test_geometries_the_grouped_products_do_not_tile_cpu(fmt, act, h, inter, h_out):
+    with pytest.raises(ValueError, match="multiples of 128"):
+        moe.check_grouped(_experts(4, h, inter, act, fmt, h_out=h_out))
+    for ok in ("mxfp4", "nvfp4", "bf16", "w3"):
+        moe.check_grouped(_experts(4, 128, 128, act, ok))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt,act,h,inter,h_out", UNTILED)
+def test_untiled_geometries_are_refused_gpu(fmt, act, h, inter, h_out):
+    ew = _experts(4, h, inter, act, fmt, h_out=h_out).to("cuda")
+    x, router = torch.randn(20, h).bfloat16().cuda(), torch.randn(4, h).bfloat16().cuda()
+    for t in (3, 20):
+        if moe.few_tokens_per_call(ew, 2, t):          # (bf16 rows of any multiple of eight run in the few-token form)
+            assert torch.isfinite(moe.layer_forward(x[:t], router, ew, 2).float()).all()
+            continue
+        with pytest.raises(ValueError, match="multiples of 128"):
+            moe.layer_forward(x[:t], router, ew, 2)
+    assert nv.read_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [1, 16, 40])
+def test_three_bit_layers_are_grouped_ones_gpu(t):
+    g = torch.Generator().manual_seed(t)
+    ew = _experts(8, 256, 128, "swiglu", "w3").to("cuda")
+    x, router, shared = (torch.randn(n, 256, generator=g).bfloat16().cuda() for n in (t, 8, t))
+    assert not moe.few_tokens_per_call(ew, 2, t)
+    ids, w = moe.route(gemm.linear_bf16(x, router, epilogue=gemm.EPI_STORE_F32), 2)
+    assert torch.equal(moe.layer_forward(x, router, ew, 2, shared=shared), moe.experts_forward(x, ids, w, ew, shared=shared))
+    assert nv.read_status() == 0
