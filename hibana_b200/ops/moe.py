@@ -546,6 +546,9 @@ def layer_forward(x: torch.Tensor, router: torch.Tensor, ew: ExpertWeights, topk
     for other in (router, rx, w1, sel_bias, shared):
         if other is not None and other.get_device() != dev:
             raise ValueError("layer_forward: operands on different devices")
+    if ew.fmt == "nvfp4" and not ew.fc1.gscale.shape == ew.fc2.gscale.shape == (e,):
+        raise ValueError(f"layer_forward: NVFP4 experts carry one scale each, {e}, got {tuple(ew.fc1.gscale.shape)} and "
+                         f"{tuple(ew.fc2.gscale.shape)}")
     most = few_tokens_per_call(ew, topk, t)
     if not nv.use_native(x):
         ids, w = route_ref(rx.float() @ router.float().t(), topk, sigmoid=sigmoid, sel_bias=sel_bias, renorm=renorm, scale=scale)

@@ -110,3 +110,17 @@ def test_three_bit_layers_are_grouped_ones_gpu(t):
     ids, w = moe.route(gemm.linear_bf16(x, router, epilogue=gemm.EPI_STORE_F32), 2)
     assert torch.equal(moe.layer_forward(x, router, ew, 2, shared=shared), moe.experts_forward(x, ids, w, ew, shared=shared))
     assert nv.read_status() == 0
+
+
+def test_scales_of_nvfp4_experts_are_one_each_cpu():
+    """The kernels read a scale at every chosen expert's number: fewer of them are refused, not read past."""
+    import dataclasses
+    x, router = torch.randn(3, 128).bfloat16(), torch.randn(4, 128).bfloat16()
+    for which in ("fc1", "fc2"):
+        ew = _experts(4, 128, 128, "relu2", "nvfp4")
+        moe.layer_forward(x, router, ew, 2)
+        w = getattr(ew, which)
+        for scales in (w.gscale[:1], w.gscale[0], w.gscale[:3]):
+            setattr(ew, which, dataclasses.replace(w, gscale=scales))
+            with pytest.raises(ValueError, match="one scale each"):
+                moe.layer_forward(x, router, ew, 2)
