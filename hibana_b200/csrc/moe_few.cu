@@ -15,7 +15,7 @@
 // eight rows. So the weights take the 128-row side of tcgen05.mma as they lie in memory, and never pass through registers: decoding
 // FP4 there costs 0.1 instructions a weight, which bounds one token as much as sixteen (measured: 1.7 TB/s of weights).
 //
-// Activations are not quantised. With FP4 weights the tensor cores want FP4 activations, so a number becomes five of them: a block (32
+// Activations are not quantised to FP4. With FP4 weights the tensor cores want FP4 activations, so a number becomes five of them: a block (32
 // elements, 16 for NVFP4) is scaled by a power of two to 14-bit integers, X = sum_p d_p 8^p with digits d_p of -4 .. 4, which
 // e2m1 holds exactly. The digits of a row are five columns of the product (five rows of operand B, with the block's scale), and
 // the epilogue adds them up: 8^p D_p. What is lost is half a unit of X, 2^-14 to 2^-15 of the largest number of its block. An NVFP4

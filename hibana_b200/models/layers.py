@@ -505,7 +505,7 @@ class MoeLayer:
     def _takes_few(self, rows: int) -> bool:
         """Whether a call of `rows` rows runs as one few-token layer (`moe.layer_forward`): MXFP4 experts always, the other
         formats with `moe_few`, as far as the layer's width allows (`moe.few_tokens_per_call`). Off where the routing is edited between its kernels (`expert_budget`) and under
-        `stable_numerics` (the form reads unquantised activations, so a request's tokens would depend on how many rows ran
+        `stable_numerics` (the form does not quantise activations to FP4, so a request's tokens would depend on how many rows ran
         beside it)."""
         cfg, ew = cfgmod.current(), self.experts
         return ((ew.fmt == "mxfp4" or cfg.moe_few) and self.ep_size == 1 and self.experts_w3 is None and not self.calibrating
