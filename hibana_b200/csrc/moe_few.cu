@@ -347,9 +347,11 @@ __device__ __forceinline__ void make_plan(Plan& plan, int tokens, int topk) {
   __syncthreads();
 }
 
-__device__ __forceinline__ uint32_t order_key(float v) {          // orders floats as unsigned numbers; never 0
+// Orders floats as unsigned numbers, NaN in front of all; never 0. (NaN is asked for by itself: the compiler may make `b | 0x80000000` a
+// floating-point -|v|, which turns a NaN into one without the sign bit, between the positive and the negative numbers.)
+__device__ __forceinline__ uint32_t order_key(float v) {
   const uint32_t b = __float_as_uint(v);
-  return max((b & 0x80000000u) ? ~b : (b | 0x80000000u), 1u);
+  return v != v ? 0xFFFFFFFFu : (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
 // Top-k of one token by one warp, PER experts a lane. Lane j < topk returns id and weight, in descending order of score
@@ -474,7 +476,10 @@ __device__ __forceinline__ void warp_topk(const FewParams& p, const float* logit
       weight /= warp_sum(sum);
     }
   }
-  if (p.renorm) weight = weight / fmaxf(warp_sum(weight), 1e-20f);
+  if (p.renorm) {
+    const float sum = warp_sum(weight);
+    weight = weight / (sum < 1e-20f ? 1e-20f : sum);          // (fmaxf would put the bound in a NaN's place)
+  }
   weight *= p.scale;
 }
 
