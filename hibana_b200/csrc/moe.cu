@@ -24,9 +24,14 @@ constexpr int MAX_TOPK = 32;
 // (order-preserving bits of the value above the complemented index), a lane keeps the best of its PER keys, and
 // each of the top-k rounds is two warp-wide `redux.max` instructions plus a rescan by the one lane that owned the
 // winner, instead of a shuffle tree over (value, index) pairs.
+// (NaN in front of all, asked for by itself: the compiler may make `b | 0x80000000` a floating-point -|v|, after which a NaN has no sign
+// bit and stands between the positive and the negative numbers. No key is 0.)
 __device__ __forceinline__ unsigned route_key(float v) {
   const unsigned b = __float_as_uint(v);
-  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+  return v != v ? 0xFFFFFFFFu : (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float renormed(float w, float sum) {      // (fmaxf would put the bound in a NaN's place)
+  return w / (sum < 1e-20f ? 1e-20f : sum);
 }
 
 // Decode-sized routing: one CTA per token, one thread per expert. The k-th largest key is found by a 32-step bit
@@ -106,7 +111,7 @@ __global__ void __launch_bounds__(1024) moe_route_block_kernel(
   if (e < topk) {
     float wsum = 0.f;
     for (int i = 0; i < topk; ++i) wsum += s_sorted[i];       // in rank order, like the round-by-round kernel
-    const float w = (renorm ? s_sorted[e] / fmaxf(wsum, 1e-20f) : s_sorted[e]) * scale;
+    const float w = (renorm ? renormed(s_sorted[e], wsum) : s_sorted[e]) * scale;
     weights[static_cast<long long>(t) * topk + e] = w;
   }
 }
@@ -200,7 +205,7 @@ __global__ void moe_route_kernel(const float* __restrict__ logits, long long ld,
     }
   }
   if (lane < topk) {
-    const float w = (renorm ? my_w / fmaxf(wsum, 1e-20f) : my_w) * scale;
+    const float w = (renorm ? renormed(my_w, wsum) : my_w) * scale;
     ids[static_cast<long long>(t) * topk + lane] = my_id;
     weights[static_cast<long long>(t) * topk + lane] = w;
   }

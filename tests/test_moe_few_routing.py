@@ -71,3 +71,21 @@ def test_neighbours_change_the_order_of_sums_at_most_gpu(fmt, k):
     whole = moe.layer_forward(xg[:8], same, ewg, k)
     assert all(torch.equal(moe.layer_forward(xg[i:i + 1], same, ewg, k), whole[i:i + 1]) for i in range(8))
     assert nv.read_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sig", [False, True])
+@pytest.mark.parametrize("renorm", [False, True])
+@pytest.mark.parametrize("t,e", [(3, 8), (3, 200), (300, 200), (3, 600)])      # both routing kernels
+def test_route_orders_nan_as_the_plain_form_gpu(t, e, sig, renorm):
+    """One NaN logit, a row of them, NaN with either sign: ids and weights of the plain form."""
+    lg = torch.randn(t, e, generator=torch.Generator().manual_seed(e))
+    lg[0, 5] = float("nan")
+    lg[1] = float("nan")
+    lg.view(torch.int32)[2, 3] = -1
+    ids, w = moe.route(lg.cuda(), 6, sigmoid=sig, renorm=renorm)
+    ids_ref, w_ref = moe.route_ref(lg, 6, sigmoid=sig, renorm=renorm)
+    assert torch.equal(ids.cpu(), ids_ref) and torch.equal(w.cpu().isnan(), w_ref.isnan())
+    # exponential, sum of up to 600 of them, quotients
+    ok = ~w_ref.isnan()
+    assert ((w.cpu() - w_ref).abs()[ok] <= 2.0 ** -14 * w_ref[ok]).all()
