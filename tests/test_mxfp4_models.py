@@ -240,3 +240,25 @@ def test_calibration_sees_the_rows_of_short_prompts_cpu(fmt):
     for name, layer in layers.items():
         assert int(cov.experts.rows[name].sum()) == sum(map(len, samples)) * t.top_k
         assert not layer.calibrating
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("latent", [False, True])
+@pytest.mark.parametrize("fmt", ["bf16", "nvfp4", "mxfp4"])
+@pytest.mark.parametrize("rows", [1, 5, 16])
+def test_moe_layer_gpu_is_its_parts(fmt, latent, rows):
+    """The model's layer is the bits of its parts called one by one: `layer_forward` (held to 64 bits where that is tested) on the latent
+    or the hidden rows, routed on the hidden ones, and the shared expert, added inside the layer or behind the up-projection."""
+    from hibana_b200.ops import basic
+    t, layer = _layer(fmt, "cuda", latent=latent, act="relu2" if latent else "swiglu")
+    x = torch.randn(rows, t.hidden, generator=torch.Generator().manual_seed(4)).bfloat16().cuda()
+    with cfgmod.using(moe_few=True):
+        got = layer.forward(x)
+        shared = layer.shared.forward(x)
+    kw = dict(sigmoid=t.router == "sigmoid", sel_bias=layer.sel_bias, scale=t.router_scale)
+    if latent:
+        y = moe.layer_forward(layer.fc1_latent(x), layer.router.weight, layer.experts, t.top_k, route_x=x, **kw)
+        want = basic.add(layer.fc2_latent(y), shared)
+    else:
+        want = moe.layer_forward(x, layer.router.weight, layer.experts, t.top_k, shared=shared, **kw)
+    assert torch.equal(got, want) and nv.read_status() == 0
