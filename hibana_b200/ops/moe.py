@@ -468,9 +468,13 @@ def few_tokens_ok(ew: ExpertWeights, topk: int) -> bool:
     """Whether the few-token form covers a layer of any width: bf16, NVFP4 or MXFP4 experts, at most 1024 of them and 32 a token,
     with whole blocks (128 rows of FP4 weights and their scales) per expert and matrix. How many rows it takes at a width:
     `few_tokens_limit`; whether it is what a call gets: `few_tokens_per_call`."""
-    rows, k = (8, 8) if ew.fmt == "bf16" else (128, 32)
-    return (ew.fmt in _KINDS and ew.act in ("swiglu", "relu2") and ew.experts <= 1024 and topk <= 32 and ew.n1 % rows == 0
-            and ew.fc2_rows % rows == 0 and ew.hidden % k == 0 and ew.inter % k == 0)
+    return _few_covers(ew.fmt, ew.act, ew.experts, ew.hidden, ew.inter, ew.fc2_rows, topk)
+
+
+def _few_covers(fmt: str, act: str, experts: int, hidden: int, inter: int, h_out: int, topk: int) -> bool:
+    rows, k = (8, 8) if fmt == "bf16" else (128, 32)
+    return (fmt in _KINDS and act in ("swiglu", "relu2") and experts <= 1024 and topk <= 32
+            and (2 * inter if act == "swiglu" else inter) % rows == 0 and h_out % rows == 0 and hidden % k == 0 and inter % k == 0)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -493,9 +497,14 @@ def few_tokens_per_call(ew: ExpertWeights, topk: int, tokens: int) -> int:
     """Tokens that a call of the kernels takes where `layer_forward` of `tokens` rows has the few-token form, 0 where it has the
     grouped one: more than FEW_TOKENS rows, a layer that `few_tokens_ok` does not cover, or one so wide that two calls would not do
     (every call reads its experts' weights). The same on every device."""
-    if not 0 < tokens <= FEW_TOKENS or not few_tokens_ok(ew, topk):
+    return _few_per_call(ew.fmt, ew.act, ew.experts, ew.hidden, ew.inter, ew.fc2_rows, topk, tokens)
+
+
+@functools.lru_cache(maxsize=4096)
+def _few_per_call(fmt: str, act: str, experts: int, hidden: int, inter: int, h_out: int, topk: int, tokens: int) -> int:
+    if not 0 < tokens <= FEW_TOKENS or not _few_covers(fmt, act, experts, hidden, inter, h_out, topk):
         return 0
-    most = few_tokens_limit(ew.fmt, ew.hidden)
+    most = few_tokens_limit(fmt, hidden)
     return min(most, tokens) if 2 * most >= tokens else 0
 
 
@@ -545,8 +554,9 @@ def layer_forward(x: torch.Tensor, router: torch.Tensor, ew: ExpertWeights, topk
         raise ValueError(f"layer_forward: top-{topk} of {e} experts")
     if sel_bias is not None and (not sigmoid or sel_bias.shape != (e,) or sel_bias.dtype != torch.float32):
         raise ValueError("layer_forward: the selection bias is fp32, one number an expert, and goes with sigmoid scores")
-    if shared is not None and (shared.shape != (t, ew.fc2_rows) or shared.dtype != torch.bfloat16):
-        raise ValueError(f"layer_forward: bf16 shared rows {(t, ew.fc2_rows)} expected, got {shared.dtype} {tuple(shared.shape)}")
+    h_out = ew.fc2_rows
+    if shared is not None and (shared.shape != (t, h_out) or shared.dtype != torch.bfloat16):
+        raise ValueError(f"layer_forward: bf16 shared rows {(t, h_out)} expected, got {shared.dtype} {tuple(shared.shape)}")
     w1 = ew.fc1 if isinstance(ew.fc1, torch.Tensor) else ew.fc1.q
     dev = x.get_device()
     for other in (router, rx, w1, sel_bias, shared):
@@ -555,27 +565,26 @@ def layer_forward(x: torch.Tensor, router: torch.Tensor, ew: ExpertWeights, topk
     if ew.fmt == "nvfp4" and not ew.fc1.gscale.shape == ew.fc2.gscale.shape == (e,):
         raise ValueError(f"layer_forward: NVFP4 experts carry one scale each, {e}, got {tuple(ew.fc1.gscale.shape)} and "
                          f"{tuple(ew.fc2.gscale.shape)}")
-    most = few_tokens_per_call(ew, topk, t)
+    most = _few_per_call(ew.fmt, ew.act, e, ew.hidden, ew.inter, h_out, topk, t)
     if not nv.use_native(x):
         ids, w = route_ref(rx.float() @ router.float().t(), topk, sigmoid=sigmoid, sel_bias=sel_bias, renorm=renorm, scale=scale)
         return few_tokens_ref(x, ids, w, ew, shared) if most else experts_forward(x, ids, w, ew, shared=shared)
     with nv.on_device(x):
         if t == 0:
-            return torch.empty(0, ew.fc2_rows, dtype=torch.bfloat16, device=x.device)
+            return torch.empty(0, h_out, dtype=torch.bfloat16, device=x.device)
         # both forms: rows that 16-byte loads can read, a router whose rows are whole 16 bytes (zeros behind an odd width), a plain bias
         x, shared = _rows16(x), _rows16(shared)
-        rx = x if route_x is None else route_x
         pad = -router.shape[1] % 8
         if pad:
             rx, router = F.pad(rx, (0, pad)), F.pad(router, (0, pad))
-        rx, router = _rows16(rx), _rows16(router)
+        rx, router = x if route_x is None and not pad else _rows16(rx), _rows16(router)
         if sel_bias is not None:
             sel_bias = sel_bias.contiguous()
         if not most:
             ids, w = route(gemm.linear_bf16(rx, router, epilogue=gemm.EPI_STORE_F32), topk, sigmoid=sigmoid, sel_bias=sel_bias,
                            renorm=renorm, scale=scale)
             return experts_forward(x, ids, w, ew, shared=shared)
-        out = torch.empty(t, ew.fc2_rows, dtype=torch.bfloat16, device=x.device)
+        out = torch.empty(t, h_out, dtype=torch.bfloat16, device=x.device)
         score, kind = (int(sigmoid), int(renorm), scale), _KINDS[ew.fmt]
         if most == t:
             _few_launch(kind, x, rx, router, ew, topk, score, sel_bias, shared, out)
