@@ -97,7 +97,8 @@ class EngineConfig:
                                            # latent projection) run on a side stream beside the routed experts; 0 = off
     moe_few: bool = False                  # bf16 and NVFP4 MoE layers of up to 16 rows (fewer, or none, in wide layers:
                                            # moe.few_tokens_per_call) on one GPU run as one few-token layer
-                                           # (moe.layer_forward: activations in 14 bits, not FP4); MXFP4 layers always do
+                                           # (moe.layer_forward: activations in 14 bits, not FP4; bf16
+                                           # 16 bits inside instead of 8); MXFP4 layers always do
     expert_budget: int = 0                 # > 0: decode-sized MoE calls read at most this many distinct experts
     expert_keep: int = 2                   # with a budget: choices of every row that are always honoured
     # observability

@@ -6,7 +6,8 @@
 //                  128x4-swizzled blocks and shared -> TMEM by tcgen05.cp.
 //
 //   * kind mxfp4 : tcgen05.mma kind::mxf4.block_scale (e2m1 values, ue8m0 scale per 32 elements): the same tiles with half as
-//                  many scale bytes. With its quantiser: 1 x 7168 x 5120 8.0 us, 64 x 34816 x 5120 with SiLU-mul 18.5 (97 MB).
+//                  many scale bytes. From memory, behind its quantiser: 1 x 7168 x 5120 12.9 us (2.6 + 10.3), 64 x 34816 x 5120 with
+//                  SiLU-mul 26.5 (97 MB; 22.6 where the call before left the same weights in L2).
 //
 //   * kind fp8   : tcgen05.mma kind::f8f6f4 on e4m3 operands, 128-element (128-byte) K tiles; per-tensor scales
 //                  fold into alpha, a per-token scale vector (dynamic activation quantisation) into the epilogue.

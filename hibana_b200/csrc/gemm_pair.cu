@@ -1,8 +1,10 @@
 // Prefill-sized NVFP4 / MXFP4 GEMM for sm_100a on SM pairs: D[m, n] = A[m, K] * B[n, K]^T, tokens on the A side.
 //
-// (Both formats run the same kernel; an mxfp4 K tile has half as many scale bytes. 2048 x 34816 x 5120 in MXFP4 with SiLU-mul takes 131.5
-// us, 5.5 PFLOP/s; 301 x 5120 x 17408 31.6 from memory, 40 of 74 clusters: the token rows beyond 256 make a second row of tiles that
-// reads the weights again through L2, and splitting K would have the same bytes to move.)
+// (Both formats run the same kernel; an mxfp4 K tile has half as many scale bytes. 2048 x 34816 x 5120 in MXFP4 with SiLU-mul takes 131
+// us, 5.5 PFLOP/s, by itself, and 141 back to back; under the power cap of a loop of seconds a call with its quantiser takes 166
+// instead of 147. 301 x 5120 x 17408 takes 31.5 from memory, on 40 of 74 clusters: the token rows beyond 256 make a second row of
+// tiles that reads the weights again through L2. At the 12.5 TB/s below those bytes are 17 to 19 us; what the rest waits for has not
+// been measured, nor weights on the 256-row side with K split, which would move half of the bytes.)
 //
 // Two CTAs of a cluster share one 256 x 256 output tile (tcgen05 cta_group::2, M = 256): each stages its own 128 rows
 // of A and HALF of B, and the leader's MMA reads both shared memories. A 128 x 256 tile on one SM has to read

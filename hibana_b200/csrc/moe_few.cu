@@ -29,12 +29,12 @@
 // part of the experts, and add up through distributed shared memory in order.
 //
 // Measured (us a call among others, weights from memory; in brackets route / fc1 / fc2 on their own, and the time of the bytes at the copy
-// rate): 512 experts, 2560-640 SwiGLU, MXFP4, top 10: 1 token 23 (4.0 / 14 / 15.5; 4.4), 16 tokens 75 (4.4 / 50 / 36; 56); 512
-// experts, 1024-2688 squared ReLU, NVFP4, top 22, router over 4096: 4 tokens 59 (5.8 / 33 / 34; 40); 64 experts, 2048-768 SwiGLU, bf16,
-// top 8: 7 tokens 70 (3.5 / 48 / 31; 56). The products stream 5 to 6.6 TB/s while they stream. Bound by what happens before the first
-// weights can be named and between kernels: logits 4, top-k and plan 4, first tiles 2 each, from fc1's last tile to fc2's first 5, the
-// cluster's sums 3. fc2 runs on the clusters that fit (80 to 120 of 148 SMs: 120 with clusters of six on 20 output blocks). Fetching the
-// first of W2 into L2 from fc1's last tiles on made 16 tokens 2 us slower.
+// rate): 512 experts, 2560-640 SwiGLU, MXFP4, top 10: 1 token 23 (4.1 / 14 / 14; 4.4), 16 tokens 77 (4.4 / 51 / 35; 56); 512
+// experts, 1024-2688 squared ReLU, NVFP4, top 22, router over 4096: 4 tokens 60 (5.7 / 35 / 35; 40); 64 experts, 2048-768 SwiGLU, bf16,
+// top 8: 7 tokens 68 (3.6 / 50 / 31; 56). The products stream 5 to 6.6 TB/s while they stream. Bound by what happens before the first
+// weights can be named and between kernels: logits 4, top-k 2.5 and plan 1, first tiles 2 each, from fc1's last tile to fc2's first 5,
+// the cluster's sums 3. fc2 runs on the clusters that fit (80 to 120 of 148 SMs: 120 with clusters of six on 20 output blocks). Fetching the
+// first of W2 into L2 from fc1's last tiles on made 16 tokens 2 us slower (one token, whose fc1 leaves CTAs and memory idle, was not tried).
 #include <algorithm>
 #include <cstddef>
 
@@ -226,6 +226,8 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) moe_few_route_kernel(const _
     const __nv_bfloat16* xb = p.route_x + min(g + 8, p.tokens - 1) * p.ld_route;
     const bool two = p.tokens > 8;
     float acc[2][4] = {};
+    // Loads of 512 columns in flight. us at widths of 1024, 2560, 4096, 7168 (512 experts, one token): two 3.2, 5.3, 6.5, 9.9, four 3.3, 4.9,
+    // 5.7, 8.5, five 3.3, 4.0, 5.7, 8.0, eight 5.8, 6.6, 7.9, 11.6.
     constexpr int U = 5;
     for (int b0 = warp; b0 < blocks; b0 += ROUTE_WARPS * U) {
       uint4 wa[U], wb[U], va[U], vb[U];

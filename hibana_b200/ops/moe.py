@@ -307,7 +307,7 @@ def pair_rows(ew: "ExpertWeights", max_rows: int) -> bool:
     would otherwise be a 128-token tile, in geometries whose activation can be requantised in fc1's epilogue. One-CTA tiles /
     pairs, whole call: 512 experts, top 22, 1024-2688-1024, 129 tokens 603 / 511 us, 256 639 / 531, 904 867 / 560, 4096
     1910 / 697; 64 experts, top 8, 2048-768-2048 (SwiGLU), 129 tokens 108 / 79, 256 124 / 89, 904 178 / 120, 4096 551 / 236. MXFP4, 4096
-    tokens: 1747 / 668 and 535 / 227 (662 and 225 with the activations quantised by pair)."""
+    tokens: 1747 / 668 and 535 / 227 (649 and 217 since the activations are quantised by pair)."""
     return (ew.fmt in ("nvfp4", "mxfp4") and max_rows > 128 and ew.act in ("swiglu", "relu2") and ew.inter % 64 == 0
             and ew.n1 % 128 == 0 and ew.fc2_rows % 128 == 0)
 
@@ -442,8 +442,9 @@ def experts_forward(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, e
     return out
 
 
-# Tokens up to which a layer runs in csrc/moe_few.cu. Whole layers in graphs, weights from memory, few-token / grouped form: 512 experts,
-# top 10, 2560-640, shared expert, 16 tokens: NVFP4 121 / 158 us, MXFP4 117 / 172; 512 experts, top 22, 1024-2688: 229 / 258, 207 / 291.
+# Tokens up to which a layer runs in csrc/moe_few.cu. A model's layer in a graph, weights from memory, few-token / grouped form, 16 tokens:
+# 512 experts, top 10, 2560-640, shared expert NVFP4 115 / 158 us, MXFP4 113 / 154; 512 experts, top 22, latent 1024-2688 217 / 252, 188 / 246.
+# (Only one token of the latent layer in NVFP4 or bf16 is slower: 78 / 74 and 115 / 105.)
 FEW_TOKENS = 16
 _KINDS = {"bf16": 0, "nvfp4": 1, "mxfp4": 4}
 
