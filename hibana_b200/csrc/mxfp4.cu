@@ -92,7 +92,8 @@ struct Raw16 {
 
 // dst_rows (may be null; the expert-sorted buffers of a mixture-of-experts layer, m pairs of a token and one of its topk experts): pair r
 // goes to row dst_rows[r], of token r / topk or, with topk 0, of the same row of x; an entry that is negative or not below dst_count (rows
-// of the buffers, and with topk 0 of x) leaves the pair out. The other rows of the buffers (most of them, with few tokens: every expert's segment is padded to 128) are not touched.
+// of the buffers, and with topk 0 of x) leaves the pair out. The other rows of the buffers (most of them, with few tokens: every expert's
+// segment is padded to 128) are not touched.
 template <int IN, int ALIGN>
 __global__ void __launch_bounds__(QUANT_WARPS * 32, IN == kInF32 ? 9 : 12)
 quant_mxfp4_kernel(const void* __restrict__ x, long long ldx, int m, int k, int ka, uint8_t* __restrict__ q,

@@ -539,9 +539,9 @@ def layer_forward(x: torch.Tensor, router: torch.Tensor, ew: ExpertWeights, topk
 
     What the few-token form keeps of its activations: with FP4 experts x to 14 bits of the largest number of its block of 32 (NVFP4: 16;
     blocks below 2^-17 of their row share a scale), the inner activations to 14 bits of the largest of their token and expert: one that
-    is 2^14 times smaller than that is lost, which shows in outputs that do not weigh the large one (at a peak of 1000 times
-    the mean of the others 1e-2 of such an output, at 10^4 a tenth; the grouped form's FP4 activations 0.3 at any). With bf16 experts x is exact and the inner activations keep 16 bits each. An infinity in a
-    row makes all of it NaN with FP4 experts."""
+    is 2^14 times smaller than that is lost, which shows in outputs that do not weigh the large one (at a peak of 1000 times the mean
+    of the others 1e-2 of such an output, at 10^4 a tenth; the grouped form's FP4 activations 0.3 at any). With bf16 experts x is
+    exact and the inner activations keep 16 bits each. An infinity in a row makes all of it NaN with FP4 experts."""
     shape, e = x.shape, ew.experts
     if len(shape) != 2 or x.dtype != torch.bfloat16 or shape[1] != ew.hidden:
         raise ValueError(f"layer_forward: bf16 rows of width {ew.hidden} expected, got {x.dtype} {tuple(shape)}")
@@ -563,7 +563,7 @@ def layer_forward(x: torch.Tensor, router: torch.Tensor, ew: ExpertWeights, topk
     for other in (router, rx, w1, sel_bias, shared):
         if other is not None and other.get_device() != dev:
             raise ValueError("layer_forward: operands on different devices")
-    if ew.fmt == "nvfp4" and not ew.fc1.gscale.shape == ew.fc2.gscale.shape == (e,):
+    if ew.fmt == "nvfp4" and not ew.fc1.gscale.numel() == ew.fc2.gscale.numel() == e:
         raise ValueError(f"layer_forward: NVFP4 experts carry one scale each, {e}, got {tuple(ew.fc1.gscale.shape)} and "
                          f"{tuple(ew.fc2.gscale.shape)}")
     most = _few_per_call(ew.fmt, ew.act, e, ew.hidden, ew.inter, h_out, topk, t)
